@@ -376,6 +376,103 @@ nq_status_t nq_pack_nibbles(const int8_t *codes, int64_t rows, int32_t d, uint8_
 nq_status_t nq_unpack_nibbles(const uint8_t *packed, int64_t rows, int32_t d, int8_t *codes, nq_stream_t stream);
 
 /*
+ * Serving operators around the cache (no counterpart in the reference, whose models attend with
+ * torch).  q / k / v / out are [tokens, heads, head_dim] with a unit innermost stride, addressed
+ * through (stride_t, stride_h) in elements; pointers and strides are 16-byte aligned; head_dim is
+ * 64, 96 or 128; query head i reads KV head i / (q_heads / heads).  One layer's pages are
+ * [n_pages, heads, page_size, head_dim], contiguous, page_size 16, 32, 64 or 128; a page table
+ * lists the pages of a sequence's tokens in order.  Page indices outside the pool never fault:
+ * stores to them are skipped, reads are clamped into the pool.
+ *
+ * nq_norm_rope_qk: rows of q and k, optionally RMS-normed (q_weight / k_weight, fp32 or the
+ * tensors' type), rotated (split halves, table row positions[t]) and rounded once.  Queries go
+ * to q_out; keys to k_out, or, with pages, keys and values to token slots[t] = page * page_size +
+ * offset (a negative slot or one past the pool is skipped; slots should not repeat).
+ */
+typedef struct {
+  int32_t dtype, tokens, q_heads, heads, head_dim;  /* fp16, bf16 or fp32 */
+  const void *q, *k, *v;            /* v is needed with pages only */
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const void *q_weight, *k_weight;  /* [head_dim]; NULL: that tensor is not normed */
+  int32_t weight_f32;               /* 1: weights are fp32, 0: of `dtype` */
+  float eps;
+  const int32_t *positions;         /* [tokens], clamped to [0, rope_rows - 1] */
+  const float *rope_cos, *rope_sin; /* [rope_rows, head_dim/2], as for nq_compress_layers */
+  int32_t rope_rows;
+  void *q_out, *k_out;              /* k_out is not used with pages */
+  int64_t qo_stride_t, qo_stride_h, ko_stride_t, ko_stride_h;
+  void *k_pages, *v_pages;          /* one layer's pages, or NULL both */
+  int32_t n_pages, page_size;
+  const int32_t *slots;             /* [tokens] */
+} nq_norm_rope_params_t;
+nq_status_t nq_norm_rope_qk(const nq_norm_rope_params_t *params, nq_stream_t stream);
+
+/*
+ * Causal attention of packed sequences: the queries of sequence i are rows seq_starts[i] ..
+ * seq_starts[i+1] of q, its keys rows k_starts[i] .. k_starts[i+1] of k / v.  The last query
+ * stands at the last key (query r of nq sees keys 0 .. nk - nq + r), so keys may start before the
+ * queries.  A query that sees no key gets a zero row (lse -inf).  Starts are ascending device
+ * int32, clamped to the tensors.  Keys a query does not see never reach its output, whatever
+ * their bits.  fp16 or bf16; the softmax weights are rounded to that type for the second product,
+ * sums are fp32.
+ */
+typedef struct {
+  int32_t dtype, n_seqs, q_tokens, k_tokens, q_heads, heads, head_dim;
+  const void *q, *k, *v;
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const int32_t *seq_starts, *k_starts; /* [n_seqs + 1] */
+  float scale;                          /* logit scale; 0 = 1/sqrt(head_dim) */
+  void *out;
+  int64_t o_stride_t, o_stride_h;
+  float *lse;                           /* optional fp32 [q_tokens, q_heads]: log of the softmax sum */
+} nq_attend_prompt_params_t;
+nq_status_t nq_attend_prompt(const nq_attend_prompt_params_t *params, nq_stream_t stream);
+
+/*
+ * Decode attention over pages, one query token per sequence: sequence b attends to the first
+ * prefix_len tokens of prefix_table, which the whole batch shares and which are read once for
+ * all of it, and then to the first lens[b] tokens of its own table.  A sequence with neither gets
+ * a zero row.  What a page holds past the last token never reaches an output.  fp16 or bf16.
+ */
+typedef struct {
+  int32_t dtype, batch, q_heads, heads, head_dim, n_pages, page_size;
+  const void *q;                /* [batch, q_heads, head_dim] */
+  int64_t q_stride_b, q_stride_h;
+  const void *k_pages, *v_pages;
+  const int32_t *tables;        /* [batch, table_width] */
+  int32_t table_width;
+  const int32_t *lens;          /* [batch], clamped to [0, max_len] */
+  int32_t max_len;              /* bound on lens, at most table_width * page_size */
+  const int32_t *prefix_table;  /* [ceil(prefix_len / page_size)] */
+  int32_t prefix_len;
+  float scale;                  /* 0 = 1/sqrt(head_dim) */
+  void *out;
+  int64_t o_stride_b, o_stride_h;
+} nq_attend_pages_params_t;
+size_t nq_attend_pages_workspace_size(const nq_attend_pages_params_t *params);
+nq_status_t nq_attend_pages(const nq_attend_pages_params_t *params, void *workspace, size_t workspace_bytes,
+                            nq_stream_t stream);
+
+/*
+ * Moves between the pages of a pool [layers, n_pages, heads, page_size, head_dim] (K and V alike,
+ * contiguous, row_bytes = bytes of one row, a multiple of 16), all layers in one launch.
+ *   nq_copy_pages     page dst[i] = page src[i]; no dst page may be a src page or another dst.
+ *   nq_compact_pages  token j of dst_tables[b] = token kept_idx[b, j] of tables[b], j <
+ *                     min(kept_count[b], max_kept): what nq_select_keep kept, moved to the front of
+ *                     fresh pages.  Destination pages are pages of no source table.
+ * Entries outside the pool or the table are skipped.
+ */
+typedef struct {
+  void *k_pages, *v_pages;
+  int32_t layers, n_pages, heads, page_size, row_bytes;
+} nq_pool_t;
+nq_status_t nq_copy_pages(const nq_pool_t *pool, const int32_t *src, const int32_t *dst, int32_t n,
+                          nq_stream_t stream);
+nq_status_t nq_compact_pages(const nq_pool_t *pool, int32_t batch, const int32_t *tables, int32_t table_width,
+                             const int32_t *kept_idx, int64_t idx_stride, const int32_t *kept_count,
+                             int32_t max_kept, const int32_t *dst_tables, int32_t dst_width, nq_stream_t stream);
+
+/*
  * Device-side failure reporting (no counterpart in the reference, which has no device code).
  *
  * Every device-side wait in this library (the tensor-core scorer's waits on TMA and MMA

@@ -21,10 +21,11 @@ from .pipeline import (  # noqa: F401
 )
 from .layout import CompressedKVCache, CompressedLayer  # noqa: F401
 from .integrations.huggingface import nexusquant_evict, _EVICT_PRESETS  # noqa: F401
+from .paging import PagePool, PageBatch, PoolExhausted  # noqa: F401
 from . import kernels  # noqa: F401
 
 __all__ = [
     "NexusQuantSimple", "NexusQuantQuantOnly", "NexusQuantEvict", "NexusQuantEvictTruncate",
     "compress_kv_cache", "compress_cache_layers", "nexusquant_evict", "CompressedKVCache",
-    "CompressedLayer", "kernels",
+    "CompressedLayer", "PagePool", "PageBatch", "PoolExhausted", "kernels",
 ]

@@ -135,4 +135,69 @@ size_t attend_workspace_bytes(int batch, int q_heads, int splits);
 cudaError_t attend_take_error(unsigned int* bits, cudaStream_t s);  // read and clear its wait-error word
 cudaError_t launch_attend(const AttendArgs& a, int fmt_k, int fmt_v, void* ws, cudaStream_t s);
 
+// norm + rotation of queries and keys, store into pages (nq_rope.cu)
+struct NormRopeArgs {
+  int32_t tokens, q_heads, heads, head_dim;
+  const void *q, *k, *v;  // v nullptr: no values to store
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const void *q_weight, *k_weight;  // nullptr: no norm
+  int32_t weight_f32;               // weights are fp32 (else the tensors' type)
+  float eps;
+  const int32_t* positions;
+  const float *rope_cos, *rope_sin;
+  int32_t rope_rows;  // positions are clamped to [0, rope_rows - 1] before indexing the tables
+  void *q_out, *k_out;
+  int64_t qo_stride_t, qo_stride_h, ko_stride_t, ko_stride_h;
+  void *k_pages, *v_pages;
+  int32_t n_pages, page_shift;
+  const int32_t* slots;
+};
+cudaError_t launch_norm_rope(const NormRopeArgs& a, int dtype, cudaStream_t s);
+
+// moves between cache pages (nq_pool.cu)
+struct PoolArgs {
+  void *k, *v;            // [layers, n_pages, heads, page, head_dim]
+  int32_t layers, n_pages, heads, page_shift;
+  int32_t row_vecs;       // 16-byte pieces of one row
+  int32_t page_vecs;      // and of one page of all heads
+};
+struct CompactArgs {
+  const int32_t* tables;      // [batch, width]
+  const int32_t* kept_idx;    // [batch, idx_stride]
+  const int32_t* kept_count;  // [batch] or nullptr = max_kept
+  const int32_t* dst_tables;  // [batch, dst_width]
+  int32_t batch, width, dst_width, max_kept;
+  int64_t idx_stride;
+};
+cudaError_t launch_copy_pages(const PoolArgs& a, const int32_t* src, const int32_t* dst, int n, cudaStream_t s);
+cudaError_t launch_compact_pages(const PoolArgs& a, const CompactArgs& c, cudaStream_t s);
+
+// causal attention of packed prompts (nq_prompt.cu)
+struct PromptArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;  // [q_tokens, q_heads] or nullptr
+  int32_t n_seqs, q_tokens, k_tokens, q_heads, heads, head_dim;
+  const int32_t *starts, *k_starts;  // [n_seqs + 1]
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, o_stride_t, o_stride_h;
+  float scale;
+};
+cudaError_t launch_prompt(const PromptArgs& a, int dtype, cudaStream_t s);
+
+// decode attention over pages with a shared prefix (nq_decode.cu)
+struct DecodeArgs {
+  const void *q, *k_pages, *v_pages;
+  void* out;
+  int32_t batch, q_heads, heads, head_dim, n_pages, page_shift;
+  const int32_t* tables;  // [batch, width]
+  const int32_t* lens;    // [batch]
+  int32_t width, max_len;
+  const int32_t* prefix_table;  // [ceil(prefix_len / page)]
+  int32_t prefix_len;
+  int64_t q_stride_b, q_stride_h, o_stride_b, o_stride_h;
+  float scale;
+};
+size_t decode_workspace_bytes(const DecodeArgs& a);
+cudaError_t launch_decode(const DecodeArgs& a, int dtype, void* ws, cudaStream_t s);
+
 }  // namespace nq

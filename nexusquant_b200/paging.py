@@ -1,0 +1,212 @@
+"""A pool of fp16 / bf16 / fp32 cache pages shared by many sequences, before or without compression.
+
+``PagePool`` holds K and V of every layer as [layers, n_pages, heads, page_size, head_dim] and does
+the bookkeeping on the host: which pages a sequence's tokens are in, and how many sequences use a
+page.  The device work is in nexusquant_b200.kernels:
+
+    pool = PagePool(n_layers=32, n_pages=4096, heads=8, head_dim=128)
+    seq = pool.add()
+    slots = pool.extend(seq, n)                      # places for n new tokens
+    norm_rope_qk(q, k, pos, v=v, k_pages=pool.k[l], v_pages=pool.v[l], slots=slots)   # per layer
+    pool.compact([seq], kept_idx, kept_count)        # evict what select_keep did not keep
+    children = pool.fork(seq, 8)                     # full pages shared, the last one copied
+    batch = pool.batch(children)                     # tables, and the prefix they share
+    pool.attend(q, l, batch)                         # the shared prefix is read once
+    pool.free(seq)
+
+All device work goes to the current stream; a page that is freed may be handed out again at once,
+so use one stream for a pool or order the streams yourself.
+"""
+from __future__ import annotations
+
+import heapq
+from dataclasses import dataclass
+from typing import Dict, List, Optional, Sequence
+
+import torch
+
+from . import kernels as K
+
+
+class PoolExhausted(RuntimeError):
+    """The pool has fewer free pages than the call needs; nothing was changed."""
+
+
+@dataclass
+class PageBatch:
+    """Page tables of a batch of sequences: own pages after ``prefix_len`` shared tokens."""
+    tables: torch.Tensor                  # int32 [b, width]
+    lens: torch.Tensor                    # int32 [b], own tokens
+    max_len: int
+    prefix_table: Optional[torch.Tensor]  # int32, pages of the shared tokens
+    prefix_len: int
+
+
+@dataclass
+class _Sequence:
+    pages: List[int]
+    length: int
+
+
+class PagePool:
+    def __init__(self, n_layers: int, n_pages: int, heads: int, head_dim: int, *, page_size: int = 16,
+                 dtype: torch.dtype = torch.float16, device="cuda"):
+        if n_layers <= 0 or n_pages <= 0 or heads <= 0:
+            raise ValueError("n_layers, n_pages and heads must be positive")
+        if page_size not in K.PAGE_SIZES:
+            raise ValueError(f"page size must be one of {K.PAGE_SIZES} (got {page_size})")
+        if head_dim not in (64, 96, 128):
+            raise ValueError(f"head_dim must be 64, 96 or 128 (got {head_dim})")
+        shape = (n_layers, n_pages, heads, page_size, head_dim)
+        self.k = torch.empty(shape, dtype=dtype, device=device)
+        self.v = torch.empty(shape, dtype=dtype, device=device)
+        self.page_size = page_size
+        self.n_pages = n_pages
+        self._free = list(range(n_pages))  # a heap: the lowest free page is handed out first
+        self._uses = [0] * n_pages
+        self._seqs: Dict[int, _Sequence] = {}
+        self._next = 0
+
+    # ------------------------------------------------------------- bookkeeping
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, seq: int) -> int:
+        return self._get(seq).length
+
+    def pages(self, seq: int) -> List[int]:
+        return list(self._get(seq).pages)
+
+    def _get(self, seq: int) -> _Sequence:
+        if seq not in self._seqs:
+            raise ValueError(f"sequence {seq} is not in the pool")
+        return self._seqs[seq]
+
+    def _take(self, n: int) -> List[int]:
+        if n > len(self._free):
+            raise PoolExhausted(f"{n} pages wanted, {len(self._free)} of {self.n_pages} free")
+        got = [heapq.heappop(self._free) for _ in range(n)]
+        for p in got:
+            self._uses[p] = 1
+        return got
+
+    def _drop(self, pages: Sequence[int]) -> None:
+        for p in pages:
+            self._uses[p] -= 1
+            if self._uses[p] == 0:
+                heapq.heappush(self._free, p)
+
+    def _new(self, pages: List[int], length: int) -> int:
+        seq = self._next
+        self._next += 1
+        self._seqs[seq] = _Sequence(pages, length)
+        return seq
+
+    def _ints(self, v: Sequence[int]) -> torch.Tensor:
+        t = torch.tensor(v, dtype=torch.int32)
+        if t.numel() and self.k.is_cuda:
+            t = t.pin_memory()
+        return t.to(self.k.device, non_blocking=True)
+
+    # --------------------------------------------------------------- sequences
+    def add(self) -> int:
+        """A new, empty sequence."""
+        return self._new([], 0)
+
+    def extend(self, seq: int, n: int) -> torch.Tensor:
+        """Reserve the next ``n`` tokens of a sequence; int32 [n] slots (page * page_size + offset)."""
+        if n < 0:
+            raise ValueError(f"{n} tokens")
+        s, ps = self._get(seq), self.page_size
+        s.pages += self._take(-(-(s.length + n) // ps) - len(s.pages))
+        slots = [s.pages[t // ps] * ps + t % ps for t in range(s.length, s.length + n)]
+        s.length += n
+        return self._ints(slots)
+
+    def fork(self, seq: int, copies: int = 1) -> List[int]:
+        """``copies`` sequences with the same tokens.  Full pages are shared; a partly filled last
+        page is copied for each (all layers, one launch), so every one can be extended."""
+        if copies < 0:
+            raise ValueError(f"{copies} copies")
+        s, ps = self._get(seq), self.page_size
+        full, part = s.length // ps, s.length % ps
+        fresh = self._take(copies if part else 0)
+        if fresh:
+            try:
+                K.copy_pages(self.k, self.v, torch.tensor([s.pages[full]] * copies, dtype=torch.int32),
+                             torch.tensor(fresh, dtype=torch.int32))
+            except Exception:
+                self._drop(fresh)
+                raise
+        out = []
+        for i in range(copies):
+            for p in s.pages[:full]:
+                self._uses[p] += 1
+            out.append(self._new(s.pages[:full] + fresh[i:i + 1], s.length))
+        return out
+
+    def free(self, seq: int) -> None:
+        """Forget a sequence; pages that no other sequence uses become free."""
+        self._drop(self._get(seq).pages)
+        del self._seqs[seq]
+
+    def compact(self, seqs: Sequence[int], kept_idx: torch.Tensor, kept_count: Optional[torch.Tensor] = None) -> None:
+        """Evict: keep tokens kept_idx[i, :kept_count[i]] (ascending, as select_keep returns them) of
+        sequence seqs[i].  They move to the front of fresh pages, all layers in one launch, and the
+        old pages are dropped (pages shared with a fork stay with the fork).  Reads kept_count (a
+        host synchronisation)."""
+        seqs = list(seqs)
+        if len(set(seqs)) < len(seqs):
+            raise ValueError("a sequence is given twice")
+        if kept_idx.dim() != 2 or kept_idx.shape[0] != len(seqs):
+            raise ValueError(f"kept_idx must be [{len(seqs)}, tokens]")
+        if not seqs:
+            return
+        counts = [kept_idx.shape[1]] * len(seqs) if kept_count is None else [int(c) for c in kept_count.tolist()]
+        old = [self._get(s) for s in seqs]
+        if len(counts) != len(seqs) or any(not 0 <= c <= min(o.length, kept_idx.shape[1]) for c, o in zip(counts, old)):
+            raise ValueError("kept_count must be within the sequences and kept_idx")
+        ps = self.page_size
+        need = [-(-c // ps) for c in counts]
+        fresh = self._take(sum(need))
+        new, at = [], 0
+        for m in need:
+            new.append(fresh[at:at + m])
+            at += m
+        if max(counts) > 0:
+            try:
+                K.compact_pages(self.k, self.v, self._padded([o.pages for o in old]), kept_idx, self._ints(counts),
+                                self._padded(new), max_kept=max(counts))
+            except Exception:
+                self._drop(fresh)
+                raise
+        for s, pages, c in zip(old, new, counts):
+            self._drop(s.pages)
+            s.pages, s.length = pages, c
+
+    # --------------------------------------------------------------- attention
+    def _padded(self, rows: Sequence[Sequence[int]]) -> torch.Tensor:
+        width = max((len(r) for r in rows), default=0)
+        flat = [p for r in rows for p in list(r) + [0] * (width - len(r))]
+        return self._ints(flat).view(len(rows), width)
+
+    def batch(self, seqs: Sequence[int]) -> PageBatch:
+        """Tables of a decoding batch.  The pages that all sequences start with, full in each, are
+        its shared prefix (with a single sequence there is none)."""
+        ss, ps = [self._get(s) for s in seqs], self.page_size
+        shared = 0
+        if len(ss) > 1:
+            most = min(s.length // ps for s in ss)
+            while shared < most and all(s.pages[shared] == ss[0].pages[shared] for s in ss):
+                shared += 1
+        own = [s.length - shared * ps for s in ss]
+        return PageBatch(self._padded([s.pages[shared:] for s in ss]), self._ints(own), max(own, default=0),
+                         self._ints(ss[0].pages[:shared]) if shared else None, shared * ps)
+
+    def attend(self, q: torch.Tensor, layer: int, batch: PageBatch, *, scale: Optional[float] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """kernels.attend_pages of one layer: q [b, hq, d], one query token per sequence of the batch."""
+        return K.attend_pages(q, self.k[layer], self.v[layer], batch.tables, batch.lens,
+                              prefix_table=batch.prefix_table, prefix_len=batch.prefix_len, max_len=batch.max_len,
+                              scale=scale, out=out)

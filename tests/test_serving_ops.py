@@ -1,0 +1,706 @@
+"""Serving operators around the cache: norm_rope_qk, attend_prompt, attend_pages, copy_pages,
+compact_pages and PagePool, against plain implementations in 64 bits.
+
+Tolerances.  u is the unit roundoff of the tensors' type (2^-11 fp16, 2^-8 bf16, 2^-24 fp32).
+  norm + rotation: the result is rounded once (u |z|); the fp32 sum of at most 128 squares is off
+    by at most 2^-17 relative in any order, half of it after the root, and the products and the
+    table values add a few 2^-24: together below 2^-17 (|y1| + |y2|) for a pair (y1, y2).
+  attention: with B = sum_j p_j |v_j|, the output is rounded once (u |o|), the weights are rounded
+    to the tensors' type before the second product (u B; an fp16 weight below 2^-14 of the row's
+    largest is off by up to 2^-25 absolute instead, so 2^-24 sum_j |v_j| covers those), and fp32
+    logits, exponentials and sums add less than 2^-13 B at the logit sizes used here
+    (sum_i |q_i k_i| scale <= 32 in fp32 with 128 terms: at most 128 * 2^-24 * 32 = 2^-12 in the
+    worst case, and far from all roundings have one sign)."""
+import math
+
+import pytest
+import torch
+
+from nexusquant_b200 import PagePool, PoolExhausted
+from nexusquant_b200 import _native as N
+from nexusquant_b200 import kernels as K
+from nexusquant_b200.rope import host_tables
+
+DEV = "cuda:0"
+gpu = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+U = {F16: 2.0 ** -11, BF16: 2.0 ** -8, F32: 2.0 ** -24}
+
+
+def rand(shape, dtype, seed, outliers=False):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(shape, generator=g, device=DEV)
+    if outliers:
+        x[..., :4] *= 8.0
+    return x.to(dtype)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def attention_64(q, k, v, seen, scale=None):
+    """q [nq, hq, d], k / v [nk, h, d], seen [nq, nk] -> (o, tolerance, lse) in 64 bits.  Keys a row does
+    not see are left out of its sums, whatever their values."""
+    g = q.shape[1] // k.shape[1]
+    u = U[q.dtype]
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    kk, vv = (x.double().repeat_interleave(g, 1).transpose(0, 1) for x in (k, v))
+    x = torch.einsum("ihd,hjd->hij", q.double(), kk) * scale
+    x = torch.where(seen, x, -math.inf)
+    m = x.amax(-1, keepdim=True) if x.shape[-1] else x.new_full(x.shape[:2] + (1,), -math.inf)
+    m = torch.where(m == -math.inf, 0.0, m)
+    p = torch.where(seen, (x - m).exp(), 0.0)
+    total = p.sum(-1, keepdim=True)
+    p = torch.where(total > 0, p / total, 0.0)
+    vf = torch.where(vv.isfinite(), vv, 0.0)
+    o = p @ vf
+    bound = p @ vf.abs()
+    tol = u * o.abs() + (u + 2.0 ** -13) * bound + 2.0 ** -24 * vf.abs().sum(1, keepdim=True) + 2.0 ** -24
+    lse = torch.where(total[..., 0] > 0, m[..., 0] + total[..., 0].log(), -math.inf)
+    return o.transpose(0, 1), tol.transpose(0, 1), lse.transpose(0, 1)
+
+
+def assert_within(got, want, tol):
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} values off, worst {float((err / tol).nan_to_num(9e9).max()):.3g} x the bound"
+
+
+# --------------------------------------------------------------------------- norm + rotation + store
+def norm_rope_64(x, w, pos, eps, base=10000.0):
+    cos, sin = host_tables(int(pos.max()) + 1, x.shape[2], base)
+    c, s = (t.to(DEV).double()[pos.long()][:, None] for t in (cos, sin))
+    y = x.double()
+    if w is not None:
+        y = y / (y.pow(2).mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    a, b = y.chunk(2, -1)
+    z = torch.cat([a * c - b * s, b * c + a * s], -1)
+    tol = U[x.dtype] * z.abs() + 2.0 ** -17 * torch.cat([a.abs() + b.abs()] * 2, -1) + 2.0 ** -25
+    return z, tol
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("n,hq,h,norm,fused", [(1, 32, 8, True, True), (7, 8, 8, False, False), (130, 6, 2, True, False),
+                                               (33, 1, 1, True, True)])
+def test_norm_rope(dtype, d, n, hq, h, norm, fused):
+    x = rand((n, hq + 2 * h, d), dtype, n + d, outliers=True)
+    q, k, v = x[:, :hq], x[:, hq:hq + h], x[:, hq + h:]
+    if not fused:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    pos = (torch.arange(n, device=DEV, dtype=torch.int32) * 37 + 5) % 5000
+    wq, wk = (rand(d, dtype, 1), rand(d, F32, 2)) if norm else (None, None)
+    eps = 1e-5
+    # dense outputs
+    qo, ko = K.norm_rope_qk(q, k, pos, q_weight=wq, k_weight=wk, eps=eps)
+    zq, tq = norm_rope_64(q, wq, pos, eps)
+    zk, tk = norm_rope_64(k, wk, pos, eps)
+    assert_within(qo, zq, tq)
+    assert_within(ko, zk, tk)
+    # the same keys into pages; token 0 is skipped, the rest land in shuffled slots
+    page, n_pages = 16, n // 16 + 3
+    slots = torch.randperm(n_pages * page, generator=torch.Generator().manual_seed(3))[:n].to(torch.int32).to(DEV)
+    slots[0] = -1
+    kp = torch.full((n_pages, h, page, d), 7.0, dtype=dtype, device=DEV)
+    vp = kp.clone()
+    want_k, want_v = kp.clone(), vp.clone()
+    q2, none = K.norm_rope_qk(q, k, pos, q_weight=wq, k_weight=wk, eps=eps, v=v, k_pages=kp, v_pages=vp, slots=slots,
+                              rope_rows=5000)
+    assert none is None and torch.equal(q2, qo)
+    s = slots[1:].long()
+    want_k[s // page, :, s % page] = ko[1:]
+    want_v[s // page, :, s % page] = v[1:]
+    assert torch.equal(kp, want_k) and torch.equal(vp, want_v)
+
+
+@gpu
+def test_norm_rope_one_side_and_zero_rows():
+    """A norm on the queries alone, an all-zero row, positions past the table (clamped), n = 0."""
+    q, k = rand((5, 4, 64), F16, 0), rand((5, 2, 64), F16, 1)
+    q[2] = 0
+    pos = ints([0, 1, 2, 3, 4])
+    w = rand(64, F16, 2)
+    qo, ko = K.norm_rope_qk(q, k, pos, q_weight=w)
+    assert_within(qo, *norm_rope_64(q, w, pos, 1e-6))
+    assert_within(ko, *norm_rope_64(k, None, pos, 1e-6))
+    assert (qo[2] == 0).all()
+    far = ints([0, 1, 2, 3, 1 << 30])
+    a, _ = K.norm_rope_qk(q, k, far, rope_rows=8)
+    rows = K.TABLES.get(torch.device(DEV), 64, 10000.0, 8)[0].shape[0]
+    b, _ = K.norm_rope_qk(q, k, ints([0, 1, 2, 3, rows - 1]), rope_rows=8)
+    assert torch.equal(a, b)
+    e, f = K.norm_rope_qk(q[:0], k[:0], pos[:0])
+    assert e.shape == (0, 4, 64) and f.shape == (0, 2, 64)
+
+
+# --------------------------------------------------------------------------- prompts
+def prompt_case(lens, klens, hq, h, d, dtype, seed=0, fused=False):
+    n, m = sum(lens), sum(klens)
+    if fused:
+        x = rand((n, hq + 2 * h, d), dtype, seed, outliers=True)
+        q, k, v = x[:, :hq], x[:, hq:hq + h], x[:, hq + h:]
+    else:
+        q, k, v = rand((n, hq, d), dtype, seed), rand((m, h, d), dtype, seed + 1, outliers=True), rand((m, h, d), dtype, seed + 2)
+    at, atk = [0], [0]
+    for a, b in zip(lens, klens):
+        at.append(at[-1] + a)
+        atk.append(atk[-1] + b)
+    return q, k, v, at, atk
+
+
+def causal(nq, nk):
+    i, j = torch.arange(nq, device=DEV), torch.arange(nk, device=DEV)
+    return j[None] <= (nk - nq + i)[:, None]
+
+
+def check_prompt(got, lse, q, k, v, at, atk, scale=None):
+    for a, b, c, d in zip(at, at[1:], atk, atk[1:]):
+        o, tol, ls = attention_64(q[a:b], k[c:d], v[c:d], causal(b - a, d - c), scale)
+        assert_within(got[a:b], o, tol)
+        if lse is not None:
+            assert torch.equal(lse[a:b] == -math.inf, ls == -math.inf)
+            fin = ls > -math.inf
+            # the logits' fp32 error, as in the weights' bound
+            assert ((lse[a:b].double() - ls)[fin].abs() <= 2.0 ** -12 * (1 + ls[fin].abs())).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("lens", [[1], [5, 0, 1, 300], [128], [129, 127], [256], [257, 40], [640]])
+def test_prompt_lengths(dtype, d, lens):
+    q, k, v, at, atk = prompt_case(lens, lens, 4, 2, d, dtype, seed=sum(lens))
+    out, lse = K.attend_prompt(q, k, v, ints(at), return_lse=True)
+    check_prompt(out, lse, q, k, v, at, atk)
+
+
+@gpu
+@pytest.mark.parametrize("hq,h", [(1, 1), (3, 1), (5, 5), (14, 2), (8, 1), (16, 1), (40, 8), (64, 2), (200, 1)])
+def test_prompt_head_groups(hq, h):
+    lens = [77, 150]
+    q, k, v, at, atk = prompt_case(lens, lens, hq, h, 64, F16, seed=hq)
+    out, lse = K.attend_prompt(q, k, v, ints(at), return_lse=True)
+    check_prompt(out, lse, q, k, v, at, atk)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens,klens", [([1, 1], [1000, 3]), ([100], [700]), ([3, 200, 64], [515, 200, 65]),
+                                        ([17], [4097]), ([300, 4], [260, 0]), ([9], [0]), ([260], [3])])
+def test_prompt_keys_before_queries(dtype, lens, klens):
+    """Later chunks (keys start before the queries), and queries that see no key at all (zeros, -inf)."""
+    q, k, v, at, atk = prompt_case(lens, klens, 8, 2, 128, dtype, seed=sum(klens))
+    out, lse = K.attend_prompt(q, k, v, ints(at), k_starts=ints(atk), return_lse=True)
+    check_prompt(out, lse, q, k, v, at, atk)
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[2000], [1500, 700, 33]])
+def test_prompt_long_strided(lens):
+    q, k, v, at, atk = prompt_case(lens, lens, 8, 2, 128, F16, seed=5, fused=True)
+    assert not q.is_contiguous()
+    out = K.attend_prompt(q, k, v, ints(at), scale=0.05)
+    check_prompt(out, None, q, k, v, at, atk, scale=0.05)
+    assert torch.equal(out, K.attend_prompt(q, k, v, ints(at), scale=0.05))  # fixed order of sums
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_prompt_unseen_values_do_not_reach_a_row(dtype, d, bad):
+    """NaN and infinities in the keys and values of another sequence, and of later tokens of the same one."""
+    lens, klens = [70, 300, 20], [70, 333, 20]
+    q, k, v, at, atk = prompt_case(lens, klens, 4, 2, d, dtype, seed=9)
+    ref = K.attend_prompt(q, k, v, ints(at), k_starts=ints(atk))
+    k2, v2 = k.clone(), v.clone()
+    # the last sequence, and from the second one's key 240 on (seen by its queries 207 and later)
+    for x in (k2, v2):
+        x[atk[2]:] = bad
+        x[atk[1] + 240:atk[2]] = bad
+    out = K.attend_prompt(q, k2, v2, ints(at), k_starts=ints(atk))
+    clean = at[1] + 240 - (klens[1] - lens[1])
+    assert torch.equal(out[:clean], ref[:clean])
+    assert not out[clean:].isfinite().all(dim=-1).any()
+
+
+@gpu
+@pytest.mark.parametrize("bad,key", [(math.nan, 140), (math.inf, 129), (-math.inf, 255), (math.inf, 3)])
+def test_prompt_seen_values_do(bad, key):
+    """One value that is not finite reaches exactly the rows that see it, in its own dimension."""
+    q, k, v, at, atk = prompt_case([256], [256], 2, 1, 128, F16, seed=11)
+    v[key, 0, 5] = bad
+    o, tol, _ = attention_64(q, k, v, causal(256, 256))
+    out = K.attend_prompt(q, k, v, ints(at))
+    rows = torch.arange(256, device=DEV) >= key
+    col = out[rows][:, :, 5]
+    assert col.isnan().all() if math.isnan(bad) else (col == bad).all()
+    rest = out.clone()
+    rest[:, :, 5][rows] = o[:, :, 5][rows].to(F16)
+    assert_within(rest, o, tol)
+
+
+@gpu
+def test_prompt_extreme_logits():
+    """Rows whose logits span hundreds: the running maximum moves through the whole row."""
+    n = 700
+    q, k, v = rand((n, 2, 64), F16, 1), rand((n, 1, 64), F16, 2), rand((n, 1, 64), F16, 3)
+    k = (k.float() * torch.linspace(0.01, 12.0, n, device=DEV)[:, None, None]).half()
+    out = K.attend_prompt(q, k, v, ints([0, n]), scale=1.0)
+    o, tol, _ = attention_64(q, k, v, causal(n, n), 1.0)
+    # logits of a few hundred: their fp32 error (64 terms, |sum| up to 600) reaches 64 * 2^-24 * 600 = 2^-9.
+    tol = tol + 2.0 ** -8 * (tol / U[F16])
+    assert_within(out, o, tol)
+
+
+@gpu
+def test_prompt_far_strides():
+    """Key and value rows more than 2^31 elements apart from the first."""
+    n, step = 300, 1 << 23
+    big = torch.empty(n * step, dtype=F16, device=DEV)
+    k = big.as_strided((n, 1, 64), (step, 64, 1))
+    v = big[64:].as_strided((n, 1, 64), (step, 64, 1))
+    q = rand((n, 2, 64), F16, 0)
+    k.copy_(rand((n, 1, 64), F16, 1))
+    v.copy_(rand((n, 1, 64), F16, 2))
+    out = K.attend_prompt(q, k, v, ints([0, n]))
+    o, tol, _ = attention_64(q, k, v, causal(n, n))
+    assert_within(out, o, tol)
+
+
+@gpu
+def test_prompt_broadcast_heads_and_other_stream():
+    """Keys expanded over heads (stride 0); a call on a side stream; rows of out= that are a view."""
+    n = 200
+    q, k1, v = rand((n, 8, 128), BF16, 0), rand((n, 1, 128), BF16, 1), rand((n, 4, 128), BF16, 2)
+    k = k1.expand(n, 4, 128)
+    o, tol, _ = attention_64(q, k, v, causal(n, n))
+    assert_within(K.attend_prompt(q, k, v, ints([0, n])), o, tol)
+    side = torch.cuda.Stream()
+    buf = torch.zeros(n, 10, 128, dtype=BF16, device=DEV)
+    at = ints([0, n])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        K.attend_prompt(q, k, v, at, out=buf[:, 1:9])
+    side.synchronize()
+    assert_within(buf[:, 1:9], o, tol)
+    assert (buf[:, 0] == 0).all() and (buf[:, 9] == 0).all()
+
+
+@gpu
+def test_prompt_empty():
+    q, k = torch.empty(0, 4, 64, dtype=F16, device=DEV), torch.empty(0, 2, 64, dtype=F16, device=DEV)
+    assert K.attend_prompt(q, k, k, ints([0])).shape == (0, 4, 64)
+    assert K.attend_prompt(q, k, k, ints([0, 0, 0])).shape == (0, 4, 64)
+
+
+# --------------------------------------------------------------------------- decoding over pages
+def decode_case(b, prefix, lens, hq, h, d, dtype, page, seed=0, fill=math.nan):
+    """Pages in shuffled order; every place that holds no token is ``fill``."""
+    width = max([-(-n // page) for n in lens] + [1])
+    pre = -(-prefix // page)
+    n_pages = pre + b * width + 2
+    g = torch.Generator().manual_seed(seed)
+    order = torch.randperm(n_pages, generator=g).to(torch.int32)
+    kp = torch.full((n_pages, h, page, d), fill, dtype=dtype, device=DEV)
+    vp = kp.clone()
+    table_p, tables = order[:pre], order[pre:pre + b * width].view(b, width)
+
+    def put(table, n, s):
+        k, v = rand((n, h, d), dtype, s, outliers=True), rand((n, h, d), dtype, s + 1)
+        t = torch.arange(n)
+        at, off = table.long()[t // page].to(DEV), (t % page).to(DEV)
+        kp[at, :, off], vp[at, :, off] = k, v
+        return k, v
+
+    shared = put(table_p, prefix, 1000 + seed)
+    own = [put(tables[i], n, 2000 + 10 * i + seed) for i, n in enumerate(lens)]
+    q = rand((b, hq, d), dtype, seed)
+    return q, kp, vp, tables.to(DEV), ints(lens), table_p.to(DEV), shared, own
+
+
+def check_decode(out, q, shared, own, scale=None):
+    for i, (k, v) in enumerate(own):
+        kk, vv = torch.cat([shared[0], k]), torch.cat([shared[1], v])
+        seen = torch.ones(1, kk.shape[0], dtype=torch.bool, device=DEV)
+        o, tol, _ = attention_64(q[i:i + 1], kk, vv, seen, scale)
+        assert_within(out[i:i + 1], o, tol)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("prefix,lens", [(0, [1]), (1, [0]), (0, [0, 40, 16, 17]), (100, [3, 0, 15, 33, 1]),
+                                         (1000, [0, 700, 129])])
+def test_decode_lengths(dtype, d, page, prefix, lens):
+    q, kp, vp, tables, ln, tp, shared, own = decode_case(len(lens), prefix, lens, 8, 2, d, dtype, page, seed=prefix)
+    out = K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=prefix, max_len=max(lens))
+    check_decode(out, q, shared, own)
+    # without the bound, and again: the same bits (fixed order of sums for given bounds)
+    again = K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=prefix, max_len=max(lens))
+    assert torch.equal(out, again)
+    check_decode(K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=prefix), q, shared, own)
+
+
+@gpu
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("hq,h", [(1, 1), (3, 1), (14, 2), (32, 8), (16, 1), (34, 2), (128, 1), (150, 1)])
+def test_decode_head_groups_and_pages(page, hq, h):
+    lens = [50, 0, 129, 64]
+    for prefix in (0, 300):
+        q, kp, vp, tables, ln, tp, shared, own = decode_case(4, prefix, lens, hq, h, 128, F16, page, seed=hq)
+        out = K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=prefix)
+        check_decode(out, q, shared, own)
+
+
+@gpu
+@pytest.mark.parametrize("b", [2, 31, 32, 33, 70])
+@pytest.mark.parametrize("dtype,d", [(F16, 128), (BF16, 128), (F16, 96), (BF16, 64)])
+def test_decode_batch_over_shared_prefix(b, dtype, d):
+    lens = [(7 * i) % 45 for i in range(b)]
+    q, kp, vp, tables, ln, tp, shared, own = decode_case(b, 2100, lens, 8, 2, d, dtype, 16, seed=b)
+    out = K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=2100, max_len=max(lens), scale=0.11)
+    check_decode(out, q, shared, own, 0.11)
+
+
+@gpu
+@pytest.mark.parametrize("fill", [math.nan, math.inf, -math.inf])
+def test_decode_places_without_tokens(fill):
+    """Whatever the pages hold past the last token stays out, for the prefix and the own tokens, in few
+    rows and in many."""
+    for b, hq in ((2, 4), (40, 16)):
+        lens = [(5 * i) % 37 for i in range(b)]
+        q, kp, vp, tables, ln, tp, shared, own = decode_case(b, 203, lens, hq, 2, 128, F16, 64, seed=3, fill=fill)
+        out = K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=203)
+        check_decode(out, q, shared, own)
+
+
+@gpu
+def test_decode_seen_nan_reaches_its_rows_only():
+    q, kp, vp, tables, ln, tp, shared, own = decode_case(40, 128, [5] * 40, 8, 2, 64, F16, 16, seed=4)
+    ref = K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=128)
+    vp[tables[7, 0].long(), :, 2] = math.nan  # a token of sequence 7 alone
+    out = K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=128)
+    others = torch.arange(40, device=DEV) != 7
+    assert torch.equal(out[others], ref[others]) and out[7].isnan().all()
+    vp[tp[3].long(), 1, 4] = math.nan  # a prefix token, KV head 1: query heads 4..7 of everyone
+    out = K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=128)
+    assert out[:, 4:].isnan().all() and torch.equal(out[others, :4], ref[others, :4])
+
+
+@gpu
+def test_decode_no_tokens_and_bad_pages():
+    q, kp, vp, tables, ln, tp, shared, own = decode_case(3, 40, [4, 4, 4], 8, 2, 128, F16, 16, seed=5, fill=0.0)
+    out = K.attend_pages(q, kp, vp, tables, ints([0, 0, 0]))
+    assert (out == 0).all()
+    assert (K.attend_pages(q, kp, vp, tables[:, :0], ints([0, 0, 0])) == 0).all()
+    assert K.attend_pages(q[:0], kp, vp, tables[:0], ln[:0], prefix_table=tp, prefix_len=40).shape == (0, 8, 128)
+    # lengths above the bound are clamped to it, page numbers outside the pool to the pool
+    a = K.attend_pages(q, kp, vp, tables, ints([99, 4, -3]), prefix_table=tp, prefix_len=40, max_len=4)
+    b = K.attend_pages(q, kp, vp, tables, ints([4, 4, 0]), prefix_table=tp, prefix_len=40, max_len=4)
+    assert torch.equal(a, b)
+    wild, wild_p = tables.clone(), tp.clone()
+    wild[0, 0], wild[1, 0], wild_p[0] = 1 << 30, -5, -9
+    assert K.attend_pages(q, kp, vp, wild, ln, prefix_table=wild_p, prefix_len=40).isfinite().all()
+    q2 = rand((40, 8, 128), F16, 1)
+    assert K.attend_pages(q2, kp, vp, wild[:1].expand(40, -1), ints([4] * 40), prefix_table=wild_p,
+                          prefix_len=40).isfinite().all()
+
+
+@gpu
+def test_decode_far_pages():
+    """Pages more than 2^31 elements into the pool."""
+    page, h, d = 64, 8, 128
+    n_pages = (1 << 31) // (page * h * d) + 40
+    kp = torch.empty((n_pages, h, page, d), dtype=F16, device=DEV)
+    vp = torch.empty_like(kp)
+    tp, tables = torch.arange(n_pages - 30, n_pages - 25), torch.arange(n_pages - 20, n_pages - 12).view(4, 2)
+    for t in (tp, tables.flatten()):
+        kp[t.to(DEV)], vp[t.to(DEV)] = rand((len(t), h, page, d), F16, 1), rand((len(t), h, page, d), F16, 2)
+
+    def rows(p, t):
+        return p[t.to(DEV)].transpose(1, 2).reshape(-1, h, d)
+
+    for b, hq in ((4, 8), (4, 64)):
+        q = rand((b, hq, d), F16, 3)
+        lens = [100, 128, 1, 60]
+        out = K.attend_pages(q, kp, vp, tables.to(DEV), ints(lens), prefix_table=tp.to(DEV), prefix_len=300)
+        check_decode(out, q, (rows(kp, tp)[:300], rows(vp, tp)[:300]),
+                     [(rows(kp, t)[:n], rows(vp, t)[:n]) for t, n in zip(tables, lens)])
+
+
+# --------------------------------------------------------------------------- moves between pages
+@gpu
+@pytest.mark.parametrize("dtype,layers,h,page,d", [(F16, 3, 8, 16, 128), (F32, 1, 2, 32, 96), (BF16, 2, 5, 128, 64)])
+def test_copy_pages(dtype, layers, h, page, d):
+    kp, vp = rand((layers, 12, h, page, d), dtype, 0), rand((layers, 12, h, page, d), dtype, 1)
+    k0, v0 = kp.clone(), vp.clone()
+    src, dst = [3, 3, 11], [0, 7, 5]
+    K.copy_pages(kp, vp, ints(src), ints(dst))
+    k0[:, dst], v0[:, dst] = k0[:, src], v0[:, src]
+    assert torch.equal(kp, k0) and torch.equal(vp, v0)
+    K.copy_pages(kp, vp, ints([]), ints([]))
+    K.copy_pages(kp, vp, ints([0, 1, 12, -1]), ints([12, -1, 2, 4]))  # outside the pool: skipped
+    assert torch.equal(kp, k0) and torch.equal(vp, v0)
+    K.copy_pages(kp[0], vp[0], torch.tensor([1]), torch.tensor([2]))  # one layer, numbers from the host
+    k0[0, 2] = k0[0, 1]
+    assert torch.equal(kp, k0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,layers,h,page,d", [(F16, 2, 8, 16, 128), (F32, 1, 3, 32, 64), (BF16, 2, 6, 64, 96)])
+@pytest.mark.parametrize("n,counts", [([40, 100, 1], [7, 64, 1]), ([130, 0, 16], [130, 0, 0])])
+def test_compact_pages(dtype, layers, h, page, d, n, counts):
+    b, width = len(n), -(-max(n) // page)
+    to = max(1, -(-max(counts) // page))
+    n_pages = b * (width + to) + 1
+    kp, vp = rand((layers, n_pages, h, page, d), dtype, 0), rand((layers, n_pages, h, page, d), dtype, 1)
+    order = torch.randperm(n_pages, generator=torch.Generator().manual_seed(2))
+    tables, dst = order[:b * width].view(b, width), order[b * width:b * (width + to)].view(b, to)
+    g = torch.Generator().manual_seed(7)
+    idx = torch.full((b, max(n)), 1 << 30, dtype=torch.int32)
+    for i in range(b):
+        idx[i, :counts[i]] = torch.randperm(n[i], generator=g)[:counts[i]].sort().values.to(torch.int32)
+    want = []
+    for p in (kp, vp):
+        w = p.clone()
+        for i in range(b):
+            for j in range(counts[i]):
+                t = int(idx[i, j])
+                w[:, dst[i, j // page], :, j % page] = p[:, tables[i, t // page], :, t % page]
+        want.append(w)
+    K.compact_pages(kp, vp, tables.to(DEV), idx.to(DEV), ints(counts), dst.to(DEV))
+    assert torch.equal(kp, want[0]) and torch.equal(vp, want[1])
+
+
+@gpu
+def test_moves_far_into_the_pool():
+    h, page, d = 8, 64, 128
+    n_pages = (1 << 31) // (page * h * d) + 8
+    kp = torch.empty((1, n_pages, h, page, d), dtype=F16, device=DEV)
+    vp = torch.empty_like(kp)
+    kp[0, -1], vp[0, -1] = rand((h, page, d), F16, 0), rand((h, page, d), F16, 1)
+    K.copy_pages(kp, vp, ints([n_pages - 1]), ints([n_pages - 3]))
+    assert torch.equal(kp[0, -3], kp[0, -1]) and torch.equal(vp[0, -3], vp[0, -1])
+    K.compact_pages(kp, vp, ints([[n_pages - 1]]), ints([[1, 5, 63]]), ints([3]), ints([[n_pages - 4]]))
+    assert torch.equal(kp[0, -4, :, :3], kp[0, -1][:, [1, 5, 63]])
+    assert torch.equal(vp[0, -4, :, :3], vp[0, -1][:, [1, 5, 63]])
+
+
+# --------------------------------------------------------------------------- the pool
+@gpu
+def test_pool_serves_a_batch():
+    """Prompt -> eviction -> forks -> decoding, every sequence's tokens checked against a dense copy."""
+    layers, h, hq, d = 2, 2, 8, 64
+    pool = PagePool(layers, 64, h, d, page_size=16, device=DEV)
+    dense = {}
+
+    def append(seq, n, seed):
+        k, v = rand((n, h, d), F16, seed), rand((n, h, d), F16, seed + 1)
+        slots = pool.extend(seq, n)
+        for l in range(layers):
+            pos = torch.arange(n, device=DEV, dtype=torch.int32)
+            _, rk = K.norm_rope_qk(k, k + l, pos, rope_rows=64)
+            K.norm_rope_qk(k, k + l, pos, v=v - l, k_pages=pool.k[l], v_pages=pool.v[l], slots=slots,
+                           rope_rows=64)
+            ok, ov = dense.get((seq, l), (rk[:0], v[:0]))
+            dense[seq, l] = torch.cat([ok, rk]), torch.cat([ov, v - l])
+
+    def check(seqs):
+        batch = pool.batch(seqs)
+        for l in range(layers):
+            q = rand((len(seqs), hq, d), F16, 99 + l)
+            out = pool.attend(q, l, batch)
+            none = tuple(t[:0] for t in dense[seqs[0], l])
+            check_decode(out, q, none, [dense[s, l] for s in seqs])
+        return batch
+
+    a = pool.add()
+    append(a, 61, 0)
+    kept = torch.tensor([[0, 1, 5, 7, 20, 21, 22, 30, 31, 33, 34, 35, 36, 37, 40, 41, 42, 43, 44, 45, 50, 51, 52, 53, 54,
+                          55, 56, 57, 58, 59, 60, 60]], dtype=torch.int32, device=DEV)
+    pool.compact([a], kept, ints([31]))
+    assert pool.length(a) == 31 and len(pool.pages(a)) == 2
+    for l in range(layers):
+        dense[a, l] = tuple(t[kept[0, :31].long()] for t in dense[a, l])
+    check([a])
+    kids = pool.fork(a, 3)
+    for s in kids:
+        for l in range(layers):
+            dense[s, l] = dense[a, l]
+    assert pool.free_pages == 64 - 2 - 3
+    append(kids[1], 1, 50)
+    append(kids[2], 18, 60)
+    batch = check([a] + kids)
+    assert batch.prefix_len == 16 and batch.lens.tolist() == [15, 15, 16, 33]
+    pool.free(a)
+    pool.free(kids[0])
+    check(kids[1:])
+    # evicting one of two sequences that share a page leaves the other alone
+    pool.compact([kids[1]], ints([[3, 9, 31]]))
+    for l in range(layers):
+        dense[kids[1], l] = tuple(t[[3, 9, 31]] for t in dense[kids[1], l])
+    check(kids[1:])
+    for s in kids[1:]:
+        pool.free(s)
+    assert pool.free_pages == 64
+
+
+def test_pool_bookkeeping():
+    pool = PagePool(1, 6, 1, 64, page_size=16, device="cpu")
+    a = pool.add()
+    assert pool.extend(a, 0).numel() == 0
+    assert pool.extend(a, 17).tolist() == list(range(17))
+    b = pool.add()
+    assert pool.extend(b, 2).tolist() == [32, 33]
+    assert pool.extend(a, 16).tolist() == list(range(17, 32)) + [48]
+    assert (pool.pages(a), pool.length(a), pool.free_pages) == ([0, 1, 3], 33, 2)
+    with pytest.raises(PoolExhausted):
+        pool.extend(b, 100)
+    assert (pool.length(b), pool.free_pages) == (2, 2)
+    # full pages only: a fork copies nothing
+    pool.extend(b, 14)
+    c, e = pool.fork(b, 2)
+    assert pool.pages(c) == pool.pages(e) == [2] and pool.free_pages == 2
+    pool.free(b)
+    pool.free(c)
+    assert pool.free_pages == 2 and pool.extend(e, 1).tolist() == [64]
+    batch = pool.batch([a, e])
+    assert (batch.prefix_len, batch.max_len, batch.lens.tolist()) == (0, 33, [33, 17])
+    assert batch.tables.tolist() == [[0, 1, 3], [2, 4, 0]]
+    pool.free(e)
+    with pytest.raises(ValueError):
+        pool.free(e)
+    with pytest.raises(ValueError):
+        pool.extend(e, 1)
+    with pytest.raises(PoolExhausted):
+        pool.fork(a, 9)  # a partly filled page each: more than there are
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        pool.fork(a, 1)
+    assert pool.free_pages == 3  # nothing was lost
+    with pytest.raises(ValueError):
+        pool.compact([a, a], torch.zeros(2, 1, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        pool.compact([a], torch.zeros(1, 50, dtype=torch.int32), torch.tensor([34]))
+    assert pool.free_pages == 3
+
+
+@pytest.mark.parametrize("kw", [dict(page_size=8), dict(page_size=24), dict(head_dim=80), dict(n_pages=0)])
+def test_pool_refuses(kw):
+    with pytest.raises(ValueError):
+        PagePool(**{**dict(n_layers=1, n_pages=4, heads=2, head_dim=64, device="cpu"), **kw})
+
+
+# --------------------------------------------------------------------------- refusals
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 2, 64, dtype=F16)
+    i = torch.zeros(5, dtype=torch.int32)
+    pages = torch.zeros(3, 2, 16, 64, dtype=F16)
+    for call in (lambda: K.norm_rope_qk(x, x, i[:4]), lambda: K.attend_prompt(x, x, x, i),
+                 lambda: K.attend_pages(x, pages, pages, i[:4, None], i[:4]),
+                 lambda: K.copy_pages(pages, pages, i, i), lambda: K.compact_pages(pages, pages, i[None], i[None], None, i[None])):
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            call()
+
+
+@gpu
+def test_refusals():
+    q, k = rand((4, 6, 64), F16, 0), rand((4, 2, 64), F16, 1)
+    pos, at = ints([0, 1, 2, 3]), ints([0, 4])
+    pages = torch.zeros(3, 2, 16, 64, dtype=F16, device=DEV)
+    t, ln = ints([[0], [1], [2], [0]]), ints([1, 1, 1, 1])
+    bad = [
+        (ValueError, lambda: K.norm_rope_qk(q[:, :5], k, pos)),                      # 5 heads over 2
+        (ValueError, lambda: K.norm_rope_qk(q[..., :32], k[..., :32], pos)),         # head_dim 32
+        (ValueError, lambda: K.norm_rope_qk(q, k.float(), pos)),
+        (TypeError, lambda: K.norm_rope_qk(q.double(), k.double(), pos)),
+        (ValueError, lambda: K.norm_rope_qk(q, k[:3], pos)),
+        (ValueError, lambda: K.norm_rope_qk(q, k, pos[:3])),
+        (ValueError, lambda: K.norm_rope_qk(q, k, pos, q_weight=rand(32, F16, 0))),
+        (ValueError, lambda: K.norm_rope_qk(q, k, pos, k_pages=pages, v_pages=pages, slots=pos)),       # no v
+        (ValueError, lambda: K.norm_rope_qk(q, k, pos, v=k, k_pages=pages, v_pages=pages)),             # no slots
+        (ValueError, lambda: K.norm_rope_qk(q, k, pos, slots=pos)),
+        (ValueError, lambda: K.norm_rope_qk(q, k, pos, v=k, k_pages=pages[:, :1], v_pages=pages[:, :1], slots=pos)),
+        (ValueError, lambda: K.norm_rope_qk(q, k, pos, v=k, k_pages=pages.bfloat16(), v_pages=pages.bfloat16(), slots=pos)),
+        (ValueError, lambda: K.norm_rope_qk(q, k, pos, q_out=q[:3])),
+        (TypeError, lambda: K.attend_prompt(q.float(), k.float(), k.float(), at)),
+        (ValueError, lambda: K.attend_prompt(q, k, k[:3], at)),
+        (ValueError, lambda: K.attend_prompt(q, k[:3], k[:3], at)),                  # fewer keys, no k_starts
+        (ValueError, lambda: K.attend_prompt(q, k, k, at, k_starts=ints([0]))),
+        (ValueError, lambda: K.attend_prompt(q, k, k, at[:0])),
+        (ValueError, lambda: K.attend_prompt(q, k, k, at, out=q[:1].expand(4, 6, 64))),
+        (ValueError, lambda: K.attend_pages(q, pages, pages[:2], t, ln)),
+        (ValueError, lambda: K.attend_pages(q[:, :5], pages, pages, t, ln)),
+        (ValueError, lambda: K.attend_pages(q, pages, pages, t[:3], ln)),
+        (ValueError, lambda: K.attend_pages(q, pages, pages, t, ln, max_len=17)),
+        (ValueError, lambda: K.attend_pages(q, pages, pages, t, ln, prefix_len=5)),
+        (ValueError, lambda: K.attend_pages(q, pages, pages, t, ln, prefix_table=ints([0]), prefix_len=17)),
+        (ValueError, lambda: K.attend_pages(q, pages.transpose(1, 2), pages.transpose(1, 2), t, ln)),
+        (ValueError, lambda: K.attend_pages(q, pages[:, :, :8].contiguous(), pages[:, :, :8].contiguous(), t, ln)),
+        (TypeError, lambda: K.attend_pages(q.float(), pages.float(), pages.float(), t, ln)),
+        (ValueError, lambda: K.copy_pages(pages, pages, ints([0, 1]), ints([2]))),
+        (ValueError, lambda: K.copy_pages(pages, pages, torch.tensor([0, 1]), torch.tensor([1, 2]))),
+        (ValueError, lambda: K.copy_pages(pages, pages, torch.tensor([0, 0]), torch.tensor([1, 1]))),
+        (ValueError, lambda: K.copy_pages(pages, pages, torch.tensor([0]), torch.tensor([3]))),
+        (ValueError, lambda: K.compact_pages(pages, pages, t, ints([[0]]), None, t)),
+        (ValueError, lambda: K.compact_pages(pages, pages, t[:1], ints([[0, 1]]), None, t[:1], max_kept=3)),
+    ]
+    for i, (kind, call) in enumerate(bad):
+        with pytest.raises(kind):
+            call()
+            pytest.fail(f"case {i} was not refused")
+
+
+def test_entry_points_refuse_without_a_gpu():
+    """Host checks of the C entry points; each returns before anything is launched."""
+    import ctypes
+    lib = N.load()
+    one = 4096  # an aligned, never used address
+
+    def rope(**kw):
+        p = N.NormRopeParams(dtype=0, tokens=2, q_heads=4, heads=2, head_dim=128, q=one, k=one, q_out=one, k_out=one,
+                             positions=one, rope_cos=one, rope_sin=one, rope_rows=8)
+        for n, v in kw.items():
+            setattr(p, n, v)
+        return lib.nq_norm_rope_qk(ctypes.byref(p), None)
+
+    assert lib.nq_norm_rope_qk(None, None) == -1
+    assert rope(tokens=0) == 0 and rope(tokens=-1) == -1 and rope(head_dim=80) == -2 and rope(dtype=3) == -1
+    assert rope(k_out=None) == -1 and rope(rope_rows=0) == -1 and rope(q=one + 8) == -6 and rope(q_stride_t=4) == -6
+    assert rope(k_pages=one) == -1 and rope(k_pages=one, v_pages=one, page_size=48) == -2
+    assert rope(k_pages=one, v_pages=one, page_size=16) == -1  # no v, no slots
+
+    def prompt(**kw):
+        p = N.AttendPromptParams(dtype=0, n_seqs=1, q_tokens=2, k_tokens=2, q_heads=4, heads=2, head_dim=128, q=one, k=one,
+                                 v=one, seq_starts=one, k_starts=one, out=one)
+        for n, v in kw.items():
+            setattr(p, n, v)
+        return lib.nq_attend_prompt(ctypes.byref(p), None)
+
+    assert lib.nq_attend_prompt(None, None) == -1
+    assert prompt(q_tokens=0) == 0 and prompt(n_seqs=0) == 0 and prompt(dtype=2) == -2 and prompt(head_dim=32) == -2
+    assert prompt(q_heads=3) == -2 and prompt(out=None) == -1 and prompt(seq_starts=None) == -1
+    assert prompt(v=one + 2) == -6 and prompt(k_stride_h=12) == -6
+
+    def pages(**kw):
+        p = N.AttendPagesParams(dtype=0, batch=1, q_heads=4, heads=2, head_dim=128, n_pages=4, page_size=16, q=one,
+                                k_pages=one, v_pages=one, tables=one, table_width=2, lens=one, max_len=32, out=one)
+        for n, v in kw.items():
+            setattr(p, n, v)
+        return lib.nq_attend_pages(ctypes.byref(p), None, 0, None)
+
+    assert lib.nq_attend_pages(None, None, 0, None) == -1 and lib.nq_attend_pages_workspace_size(None) == 0
+    assert pages(batch=0) == 0 and pages(page_size=8) == -2 and pages(max_len=33) == -1 and pages(n_pages=0) == -1
+    assert pages(prefix_len=4) == -1 and pages(q=None) == -1 and pages(out=one + 4) == -6 and pages(dtype=2) == -2
+    pool = N.Pool(one, one, 2, 4, 2, 16, 256)
+    assert lib.nq_copy_pages(None, one, one, 1, None) == -1 and lib.nq_copy_pages(ctypes.byref(pool), one, one, 0, None) == 0
+    assert lib.nq_copy_pages(ctypes.byref(pool), None, one, 1, None) == -1
+    assert lib.nq_compact_pages(ctypes.byref(pool), 1, one, 2, one, 32, None, 17, one, 1, None) == -1
+    assert lib.nq_compact_pages(ctypes.byref(pool), 1, one, 2, one, 32, None, 0, one, 1, None) == 0
+    pool.row_bytes = 24
+    assert lib.nq_copy_pages(ctypes.byref(pool), one, one, 1, None) == -6
+    pool.page_size = 20
+    assert lib.nq_copy_pages(ctypes.byref(pool), one, one, 1, None) == -2
