@@ -421,7 +421,7 @@ typedef struct {
   const void *q, *k, *v;
   int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
   const int32_t *seq_starts, *k_starts; /* [n_seqs + 1] */
-  float scale;                          /* logit scale; 0 = 1/sqrt(head_dim) */
+  float scale;                          /* logit scale, positive; 0 = 1/sqrt(head_dim) */
   void *out;
   int64_t o_stride_t, o_stride_h;
   float *lse;                           /* optional fp32 [q_tokens, q_heads]: log of the softmax sum */
@@ -445,7 +445,7 @@ typedef struct {
   int32_t max_len;              /* bound on lens, at most table_width * page_size */
   const int32_t *prefix_table;  /* [ceil(prefix_len / page_size)] */
   int32_t prefix_len;
-  float scale;                  /* 0 = 1/sqrt(head_dim) */
+  float scale;                  /* positive; 0 = 1/sqrt(head_dim) */
   void *out;
   int64_t o_stride_b, o_stride_h;
 } nq_attend_pages_params_t;
@@ -476,11 +476,13 @@ nq_status_t nq_compact_pages(const nq_pool_t *pool, int32_t batch, const int32_t
  * Device-side failure reporting (no counterpart in the reference, which has no device code).
  *
  * Every device-side wait in this library (the tensor-core scorer's waits on TMA and MMA
- * completion, the decode attention's waits on MMA completion) has an iteration limit.  A wait
+ * completion, the decode attention's waits on MMA completion, the prompt attention's on both) has an
+ * iteration limit.  A wait
  * that runs out makes its kernel stop early, release what it holds and OR a bit into a
  * per-device error word; the scores or outputs it leaves are then not valid.  nq_device_error synchronizes `stream`, stores the word in *bits (if bits is
  * not NULL), clears it, and returns NQ_ERR_TIMEOUT if any bit was set, else NQ_OK.
- * Bits: 1 = scorer wait, 2 = nq_wait_selftest, 4 = decode attention wait.
+ * Bits: 1 = scorer wait, 2 = nq_wait_selftest, 4 = decode attention wait, 8 = attend_prompt or the
+ * shared prefix of attend_pages.
  */
 nq_status_t nq_device_error(int32_t *bits, nq_stream_t stream);
 /* Test hook: one CTA waits on an mbarrier that nothing arrives on, for max_iters (1..2^20)

@@ -182,6 +182,7 @@ struct PromptArgs {
   int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, o_stride_t, o_stride_h;
   float scale;
 };
+cudaError_t prompt_take_error(unsigned int* bits, cudaStream_t s);  // read and clear its wait-error word
 cudaError_t launch_prompt(const PromptArgs& a, int dtype, cudaStream_t s);
 
 // decode attention over pages with a shared prefix (nq_decode.cu)

@@ -1,66 +1,60 @@
-// Causal attention of packed prompts: o_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys j
-// that query i sees, in one pass with a running maximum and sum.  One warp per (query, head).
-#include "../../include/nexusquant_b200.h"
-#include "nq_common.cuh"
-#include "nq_internal.h"
+// Causal attention of packed prompts: nq_tiles.cuh on row tiles of (token, head) pairs.
+#include "nq_tiles.cuh"
 
 namespace nq {
+
 namespace {
 
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f(float x, __half* p) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void from_f(float x, __nv_bfloat16* p) { *p = __float2bfloat16_rn(x); }
-
 template <typename T, int D>
-__global__ void __launch_bounds__(128) prompt_kernel(const PromptArgs a) {
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, head = blockIdx.y;
-  if (t >= a.q_tokens) return;
-  int s = 0;
-  while (s < a.n_seqs && t >= a.starts[s + 1]) ++s;
-  T* out = static_cast<T*>(a.out) + t * a.o_stride_t + head * a.o_stride_h;
-  if (s == a.n_seqs || t < a.starts[s]) return;
-  const int k0 = min(max(a.k_starts[s], 0), a.k_tokens), k1 = min(max(a.k_starts[s + 1], k0), a.k_tokens);
-  const int nq = a.starts[s + 1] - a.starts[s];
-  const int seen = k1 - k0 - nq + (t - a.starts[s]) + 1;  // keys that this query sees
-  const int kh = head / (a.q_heads / a.heads);
-  const T* q = static_cast<const T*>(a.q) + t * a.q_stride_t + head * a.q_stride_h;
-  float qv[D / 32], acc[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) { qv[i] = to_f(q[lane + 32 * i]) * a.scale; acc[i] = 0.0f; }
-  float m = -INFINITY, l = 0.0f;
-  for (int j = 0; j < seen; ++j) {
-    const T* k = static_cast<const T*>(a.k) + (int64_t)(k0 + j) * a.k_stride_t + kh * a.k_stride_h;
-    const T* v = static_cast<const T*>(a.v) + (int64_t)(k0 + j) * a.v_stride_t + kh * a.v_stride_h;
-    float x = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) x = fmaf(qv[i], to_f(k[lane + 32 * i]), x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-    const float mn = fmaxf(m, x), f = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(x - mn);
-    m = mn;
-    l = fmaf(l, f, p);
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(acc[i], f, p * to_f(v[lane + 32 * i]));
-  }
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) from_f(seen > 0 ? acc[i] / l : 0.0f, out + lane + 32 * i);
-  if (a.lse && lane == 0) a.lse[(int64_t)t * a.q_heads + head] = seen > 0 ? m + logf(l) : -INFINITY;
+cudaError_t prompt_d(const PromptArgs& p, cudaStream_t s) {
+  TileArgs a;
+  std::memset(&a, 0, sizeof(a));
+  const int group = p.q_heads / p.heads;
+  a.q_heads = p.q_heads; a.heads = p.heads;
+  a.gp = group <= kTile ? group : 1;
+  a.tq = kTile / a.gp;
+  a.units = p.q_heads / a.gp;
+  a.scale = p.scale; a.c = p.scale * kLog2e;
+  a.starts = p.starts; a.k_starts = p.k_starts; a.n_seqs = p.n_seqs; a.q_tokens = p.q_tokens; a.k_tokens = p.k_tokens;
+  a.q = p.q; a.k = p.k; a.v = p.v;
+  a.q_stride_t = p.q_stride_t; a.q_stride_h = p.q_stride_h;
+  a.k_stride_t = p.k_stride_t; a.k_stride_h = p.k_stride_h;
+  a.v_stride_t = p.v_stride_t; a.v_stride_h = p.v_stride_h;
+  a.o_stride_t = p.o_stride_t; a.o_stride_h = p.o_stride_h;
+  a.out = p.out; a.lse = p.lse;
+  CUtensorMap qm, km, vm;
+  const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)p.q_heads, (cuuint64_t)p.q_tokens};
+  const int64_t qs[2] = {p.q_stride_h, p.q_stride_t};
+  const cuuint32_t qb[3] = {64, (cuuint32_t)a.gp, (cuuint32_t)a.tq};
+  const cuuint64_t kd[3] = {(cuuint64_t)D, (cuuint64_t)p.heads, (cuuint64_t)(p.k_tokens > 0 ? p.k_tokens : 1)};
+  const int64_t ks[2] = {p.k_stride_h, p.k_stride_t}, vs[2] = {p.v_stride_h, p.v_stride_t};
+  const cuuint32_t kb[3] = {64, 1, (cuuint32_t)kTile};
+  const int type = Half16<T>::kType;
+  const bool keys = p.k_tokens > 0;  // without any the maps are never used
+  if (!tiles_map(&qm, p.q, type, 3, qd, qs, qb)) return cudaErrorInvalidValue;
+  if (!tiles_map(&km, keys ? p.k : p.q, type, 3, kd, keys ? ks : qs, kb)) return cudaErrorInvalidValue;
+  if (!tiles_map(&vm, keys ? p.v : p.q, type, 3, kd, keys ? vs : qs, kb)) return cudaErrorInvalidValue;
+  // at most this many tiles of a CTA's tokens: one partly filled tile per sequence
+  auto ctas = [&](int tok) { return ((int64_t)p.q_tokens / tok + p.n_seqs) * a.units; };
+  // two row tiles per CTA share their key tiles; a grid that does not fill the GPU that way takes
+  // one row tile per CTA, with its keys split between the streams
+  if (ctas(2 * a.tq) >= device_sms()) return run_tiles<T, D, false, false>(qm, km, vm, a, ctas(2 * a.tq), s);
+  return run_tiles<T, D, false, true>(qm, km, vm, a, ctas(a.tq), s);
 }
 
 template <typename T>
-cudaError_t run_prompt(const PromptArgs& a, cudaStream_t s) {
-  const dim3 g((a.q_tokens + 3) / 4, a.q_heads);
-  if (a.head_dim == 128) prompt_kernel<T, 128><<<g, 128, 0, s>>>(a);
-  else if (a.head_dim == 96) prompt_kernel<T, 96><<<g, 128, 0, s>>>(a);
-  else prompt_kernel<T, 64><<<g, 128, 0, s>>>(a);
-  return cudaGetLastError();
+cudaError_t prompt_t(const PromptArgs& a, cudaStream_t s) {
+  if (a.head_dim == 128) return prompt_d<T, 128>(a, s);
+  if (a.head_dim == 96) return prompt_d<T, 96>(a, s);
+  return prompt_d<T, 64>(a, s);
 }
 
 }  // namespace
 
+cudaError_t prompt_take_error(unsigned int* bits, cudaStream_t s) { return tiles_error(bits, s); }
+
 cudaError_t launch_prompt(const PromptArgs& a, int dtype, cudaStream_t s) {
-  return dtype == NQ_F16 ? run_prompt<__half>(a, s) : run_prompt<__nv_bfloat16>(a, s);
+  return dtype == NQ_F16 ? prompt_t<__half>(a, s) : prompt_t<__nv_bfloat16>(a, s);
 }
 
 }  // namespace nq

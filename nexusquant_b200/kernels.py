@@ -715,6 +715,15 @@ def _check_out(out: torch.Tensor, like: torch.Tensor) -> None:
         raise ValueError("out needs 16-byte aligned rows of contiguous elements that do not overlap")
 
 
+def _logit_scale(scale: Optional[float]) -> float:
+    """0 for the default 1 / sqrt(head_dim), else a positive number."""
+    if scale is None:
+        return 0.0
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite (got {scale})")
+    return float(scale)
+
+
 def _launch(dev: torch.device, fn: str, *args) -> None:
     """Call an entry point on ``dev``'s current stream, with ``dev`` current while it launches."""
     if torch.cuda.current_device() == dev.index:
@@ -829,7 +838,7 @@ def attend_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts:
         if k_starts.shape != seq_starts.shape:
             raise ValueError("k_starts and seq_starts must have the same shape")
         seq_starts, k_starts = _int32(seq_starts, dev), _int32(k_starts, dev)
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    q, k, v = (_rows16(t if all(t.stride()) else t.contiguous()) for t in (q, k, v))  # no broadcast rows
     if out is None:
         out = torch.empty((n, hq, d), dtype=q.dtype, device=dev)
     else:
@@ -842,7 +851,7 @@ def attend_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts:
     p.k, p.k_stride_t, p.k_stride_h = k.data_ptr(), k.stride(0), k.stride(1)
     p.v, p.v_stride_t, p.v_stride_h = v.data_ptr(), v.stride(0), v.stride(1)
     p.seq_starts, p.k_starts = seq_starts.data_ptr(), k_starts.data_ptr()
-    p.scale = 0.0 if scale is None else float(scale)
+    p.scale = _logit_scale(scale)
     p.out, p.o_stride_t, p.o_stride_h, p.lse = out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse)
     _launch(dev, "nq_attend_prompt", ctypes.byref(p))
     return (out, lse) if return_lse else out
@@ -898,7 +907,7 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     p.k_pages, p.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
     p.tables, p.table_width, p.lens, p.max_len = tables.data_ptr(), width, lens.data_ptr(), int(max_len)
     p.prefix_table, p.prefix_len = _ptr(prefix_table), int(prefix_len)
-    p.scale = 0.0 if scale is None else float(scale)
+    p.scale = _logit_scale(scale)
     p.out, p.o_stride_b, p.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
     ref = ctypes.byref(p)
     nbytes = N.load().nq_attend_pages_workspace_size(ref)

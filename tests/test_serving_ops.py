@@ -632,6 +632,8 @@ def test_refusals():
         (ValueError, lambda: K.attend_prompt(q, k, k, at, k_starts=ints([0]))),
         (ValueError, lambda: K.attend_prompt(q, k, k, at[:0])),
         (ValueError, lambda: K.attend_prompt(q, k, k, at, out=q[:1].expand(4, 6, 64))),
+        (ValueError, lambda: K.attend_prompt(q, k, k, at, scale=-1.0)),
+        (ValueError, lambda: K.attend_pages(q, pages, pages, t, ln, scale=0.0)),
         (ValueError, lambda: K.attend_pages(q, pages, pages[:2], t, ln)),
         (ValueError, lambda: K.attend_pages(q[:, :5], pages, pages, t, ln)),
         (ValueError, lambda: K.attend_pages(q, pages, pages, t[:3], ln)),
