@@ -1,68 +1,451 @@
 // Decode attention over pages: one query token per sequence attends to a prefix that the whole
-// batch shares and then to its own pages, in one pass with a running maximum and sum.  One warp
-// per (sequence, head).
-#include "../../include/nexusquant_b200.h"
-#include "nq_common.cuh"
-#include "nq_internal.h"
+// batch shares and then to its own pages.
+//
+// softmax(q K^T) V over a set of keys splits into parts: each part p gives m_p = max_j s_j,
+// l_p = sum_j 2^(s_j - m_p), o_p = sum_j 2^(s_j - m_p) v_j, and with M = max_p m_p the result is
+// sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.  So three kernels:
+//   decode_rows    up to 8 or 16 rows (the heads of one KV head of one sequence) against a range of
+//                  its own pages; with few rows in the whole batch, also against the prefix;
+//   attend_tiles   (nq_tiles.cuh, many rows) the rows of the whole batch, 128 at a time, against a
+//                  range of the prefix, whose keys and values are then read once for all of them;
+//   decode_combine the sum above, in part order.
+// The number of parts depends on the sizes given by the host alone, so results repeat bit for bit.
+#include <algorithm>
+
+#include "nq_tiles.cuh"
 
 namespace nq {
 namespace {
 
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f(float x, __half* p) { *p = __float2half_rn(x); }
-__device__ __forceinline__ void from_f(float x, __nv_bfloat16* p) { *p = __float2bfloat16_rn(x); }
+constexpr int kDecWarps = 4;
+constexpr int kDecThreads = 32 * kDecWarps;
+constexpr int kGroup = 16;       // tokens per warp step
+constexpr int kMaxParts = 256;
 
-template <typename T, int D>
-__global__ void __launch_bounds__(32) decode_kernel(const DecodeArgs a) {
-  const int lane = threadIdx.x, head = blockIdx.x, b = blockIdx.y;
-  const int kh = head / (a.q_heads / a.heads);
-  const T* q = static_cast<const T*>(a.q) + b * a.q_stride_b + head * a.q_stride_h;
-  T* out = static_cast<T*>(a.out) + b * a.o_stride_b + head * a.o_stride_h;
-  const int own = a.max_len ? min(max(a.lens[b], 0), a.max_len) : 0;
-  float qv[D / 32], acc[D / 32];
+struct DecodePlan {
+  int rows;          // rows per CTA of decode_rows: 8 or 16
+  int own_rt, own_splits;
+  int pre_rt, pre_splits;      // prefix by decode_rows (0 splits: by attend_tiles or none)
+  int tile_splits, tiles_per_split, row_tiles;
+  bool tile_split_streams;
+  int parts;         // tile_splits + pre_splits + own_splits
+};
+
+DecodePlan decode_plan(const DecodeArgs& a) {
+  DecodePlan p;
+  std::memset(&p, 0, sizeof(p));
+  const int group = a.q_heads / a.heads, sms = device_sms();
+  const int64_t pre_rows = (int64_t)a.batch * group;
+  // the prefix by rows while all rows of a KV head fit one CTA: the tiles would be nearly empty
+  const bool tiles = a.prefix_len > 0 && pre_rows > 16 && group <= kTile;
+  p.rows = group <= 8 && (tiles || a.prefix_len == 0 || pre_rows <= 8) ? 8 : 16;
+  p.own_rt = (group + p.rows - 1) / p.rows;
+  // CTAs of decode_rows resident at once; a part has at least one group per warp
+  const int64_t slots = 3ll * sms;
+  auto splits_for = [&](int64_t items, int tokens) {
+    const int most = (tokens + kGroup * kDecWarps - 1) / (kGroup * kDecWarps);
+    const int64_t want = std::max<int64_t>(1, slots / std::max<int64_t>(items, 1));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, most), kMaxParts / 4));
+  };
+  if (a.max_len > 0) p.own_splits = splits_for((int64_t)a.batch * a.heads * p.own_rt, a.max_len);
+  if (a.prefix_len > 0 && !tiles) {
+    p.pre_rt = (int)((pre_rows + p.rows - 1) / p.rows);
+    p.pre_splits = splits_for((int64_t)a.heads * p.pre_rt, a.prefix_len);
+  }
+  if (tiles) {
+    const int tq = kTile / group, key_tiles = (a.prefix_len + kTile - 1) / kTile;
+    p.tile_split_streams = a.batch <= tq;
+    const int per = p.tile_split_streams ? tq : 2 * tq;
+    p.row_tiles = (a.batch + per - 1) / per;
+    const int64_t want = std::max<int64_t>(1, sms / ((int64_t)a.heads * p.row_tiles));
+    const int splits = (int)std::min<int64_t>(std::min<int64_t>(want, key_tiles), kMaxParts / 2);
+    p.tiles_per_split = (key_tiles + splits - 1) / splits;
+    p.tile_splits = (key_tiles + p.tiles_per_split - 1) / p.tiles_per_split;
+  }
+  p.parts = p.tile_splits + p.pre_splits + p.own_splits;
+  return p;
+}
+
+// a single part of decode_rows is the result itself
+bool needs_parts(const DecodePlan& p) { return p.parts > 1 || p.tile_splits > 0; }
+
+struct DecodeWs {
+  float *m, *l, *acc;
+};
+
+template <typename T>
+struct Mma16;
+template <>
+struct Mma16<__half> {
+  static __device__ __forceinline__ void run(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+template <>
+struct Mma16<__nv_bfloat16> {
+  static __device__ __forceinline__ void run(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+        "%2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+// A warp takes 16 tokens at a time, K and V straight from the pages into MMA operands: no shared
+// memory, no barriers, 8 KB in flight per warp.  This is bound by memory (8 rows need 4 flops per
+// byte read), so the m16n8 instructions are enough and their operand layout is what matters:
+//   S = Q K^T (rows x 16 tokens): the contraction may run over the dimensions in any order that Q
+//     and K share, so lane (r, c) reads 16 bytes of token r (and r + 8) at dimensions 8 (c + 4j):
+//     two k-steps' worth of B operand.
+//   O^T = V^T P^T (dims x rows): P^T's operand is S's accumulator as it stands.  V^T's operand pairs
+//     tokens 2c, 2c + 1 of one dimension: lane (r, c) reads 16 bytes of those two tokens (and of
+//     2c + 8, 2c + 9) and interleaves them with byte permutes; the order of dimensions over the
+//     operand's rows is free.
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kDecThreads, 3) decode_rows(const DecodeArgs a, const DecodePlan p, const DecodeWs w) {
+  constexpr int KJ = D / 32;            // 16-byte chunks of a K row per lane
+  constexpr int VH = (D + 63) / 64;     // of a V row
+  constexpr int NT = ROWS / 8;          // column tiles of O^T
+  __shared__ float sm_m[kDecWarps][ROWS], sm_l[kDecWarps][ROWS], sm_f[kDecWarps][ROWS];
+  __shared__ float sm_o[kDecWarps][ROWS][D + 4];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
+  const int group = a.q_heads / a.heads;
+
+  // ---- which rows, which tokens
+  int item = blockIdx.x, n, kh, rt, seq = 0, split, splits, part;
+  const int32_t* table;
+  const int own_items = a.batch * a.heads * p.own_rt * p.own_splits;
+  const bool own = item < own_items;
+  if (own) {
+    splits = p.own_splits;
+    split = item % splits; item /= splits;
+    kh = item % a.heads; item /= a.heads;
+    rt = item % p.own_rt;
+    seq = item / p.own_rt;
+    n = min(max(a.lens[seq], 0), a.max_len);
+    table = a.tables + (int64_t)seq * a.width;
+    part = p.tile_splits + p.pre_splits + split;
+  } else {
+    item -= own_items;
+    splits = p.pre_splits;
+    split = item % splits; item /= splits;
+    kh = item % a.heads;
+    rt = item / a.heads;
+    n = a.prefix_len;
+    table = a.prefix_table;
+    part = p.tile_splits + split;
+  }
+  // row i of the CTA: its sequence and head, or none
+  auto row_of = [&](int i, int& b, int& head) {
+    const int x = rt * ROWS + i;
+    if (own) {
+      b = seq;
+      head = kh * group + x;
+      return x < group;
+    }
+    b = x / group;
+    head = kh * group + x % group;
+    return b < a.batch;
+  };
+
+  uint4 q[NT][KJ];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) { qv[i] = to_f(q[lane + 32 * i]) * a.scale; acc[i] = 0.0f; }
-  float m = -INFINITY, l = 0.0f;
-  for (int part = 0; part < 2; ++part) {
-    const int32_t* table = part ? a.tables + (int64_t)b * a.width : a.prefix_table;
-    const int n = part ? own : a.prefix_len;
-    for (int j = 0; j < n; ++j) {
-      const int page = min(max(table[j >> a.page_shift], 0), a.n_pages - 1);
-      const int64_t row = ((((int64_t)page * a.heads + kh) << a.page_shift) + (j & ((1 << a.page_shift) - 1))) * D;
-      const T* k = static_cast<const T*>(a.k_pages) + row;
-      const T* v = static_cast<const T*>(a.v_pages) + row;
-      float x = 0.0f;
+  for (int t = 0; t < NT; ++t) {
+    int b, head;
+    const bool ok = row_of(r + 8 * t, b, head);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) x = fmaf(qv[i], to_f(k[lane + 32 * i]), x);
+    for (int j = 0; j < KJ; ++j)
+      q[t][j] = ok ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.q_stride_b +
+                                                          head * a.q_stride_h) + c + 4 * j)
+                   : make_uint4(0u, 0u, 0u, 0u);
+  }
+  const float cs = a.scale * kLog2e;
+  float m[NT], l[NT], o[VH * 4][NT][4];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      const float mn = fmaxf(m, x), f = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(x - mn);
-      m = mn;
-      l = fmaf(l, f, p);
+  for (int t = 0; t < NT; ++t) {
+    m[t] = -INFINITY;
+    l[t] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(acc[i], f, p * to_f(v[lane + 32 * i]));
+    for (int i = 0; i < VH * 4; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.0f;
+  }
+
+  const int groups = (n + kGroup - 1) / kGroup, per = (groups + splits - 1) / splits;
+  const int g1 = min(groups, (split + 1) * per);
+  for (int g = split * per + warp; g < g1; g += kDecWarps) {
+    const int t0 = g * kGroup, page = min(max(__ldg(table + (t0 >> a.page_shift)), 0), a.n_pages - 1);
+    const int64_t base = ((((int64_t)page * a.heads + kh) << a.page_shift) + (t0 & ((1 << a.page_shift) - 1))) * D;
+    const T* kp = static_cast<const T*>(a.k_pages) + base;
+    const T* vp = static_cast<const T*>(a.v_pages) + base;
+    const int left = n - t0;  // tokens past the end count as zeros, whatever the page holds
+    uint4 kw[2][KJ], vw[4][VH];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+        kw[i][j] = r + 8 * i < left ? ld_stream(kp + (r + 8 * i) * D + (c + 4 * j) * 8) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int tok = 2 * c + (i & 1) + 8 * (i >> 1);
+#pragma unroll
+      for (int h = 0; h < VH; ++h)
+        vw[i][h] = tok < left && (D % 64 == 0 || h == 0 || r < 4) ? ld_stream(vp + tok * D + (r + 8 * h) * 8)
+                                                                  : make_uint4(0u, 0u, 0u, 0u);
+    }
+    float s[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) {
+        Mma16<T>::run(s[i], q[0][j].x, NT > 1 ? q[NT - 1][j].x : 0u, q[0][j].y, NT > 1 ? q[NT - 1][j].y : 0u, kw[i][j].x,
+                      kw[i][j].y);
+        Mma16<T>::run(s[i], q[0][j].z, NT > 1 ? q[NT - 1][j].z : 0u, q[0][j].w, NT > 1 ? q[NT - 1][j].w : 0u, kw[i][j].z,
+                      kw[i][j].w);
+      }
+    }
+    uint32_t pw[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float x[4] = {s[0][2 * t], s[0][2 * t + 1], s[1][2 * t], s[1][2 * t + 1]};
+      if (left < kGroup) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (2 * c + (i & 1) + 8 * (i >> 1) >= left) x[i] = -INFINITY;
+      }
+      float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      // rescale only when the maximum grew by more than 2^8 in the weights (see nq_tiles.cuh)
+      const bool grow = mx > m[t] && !((mx - m[t]) * cs <= 8.0f);
+      if (__any_sync(0xffffffffu, grow)) {
+        const float f = !grow ? 1.0f : (m[t] == -INFINITY ? 0.0f : ex2t((m[t] - mx) * cs));
+        if (grow) m[t] = mx;
+        l[t] *= f;
+        const float f0 = __shfl_sync(0xffffffffu, f, 8 * c), f1 = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+#pragma unroll
+        for (int i = 0; i < VH * 4; ++i) {
+          o[i][t][0] *= f0;
+          o[i][t][1] *= f1;
+          o[i][t][2] *= f0;
+          o[i][t][3] *= f1;
+        }
+      }
+      const float mc = m[t] == -INFINITY ? 0.0f : m[t] * cs;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = ex2t(fmaf(x[i], cs, -mc));
+      l[t] += (x[0] + x[1]) + (x[2] + x[3]);
+      pw[t][0] = Half16<T>::pack(x[0], x[1]);
+      pw[t][1] = Half16<T>::pack(x[2], x[3]);
+    }
+#pragma unroll
+    for (int h = 0; h < VH; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = j == 0 ? vw[i][h].x : j == 1 ? vw[i][h].y : j == 2 ? vw[i][h].z : vw[i][h].w;
+        const uint32_t a0 = __byte_perm(y[0], y[1], 0x5410), a1 = __byte_perm(y[0], y[1], 0x7632);
+        const uint32_t a2 = __byte_perm(y[2], y[3], 0x5410), a3 = __byte_perm(y[2], y[3], 0x7632);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) Mma16<T>::run(o[4 * h + j][t], a0, a1, a2, a3, pw[t][0], pw[t][1]);
+      }
+  }
+
+  // ---- the four warps' parts to one
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    l[t] += __shfl_xor_sync(0xffffffffu, l[t], 1);
+    l[t] += __shfl_xor_sync(0xffffffffu, l[t], 2);
+    if (c == 0) {
+      sm_m[warp][r + 8 * t] = m[t];
+      sm_l[warp][r + 8 * t] = l[t];
+    }
+#pragma unroll
+    for (int h = 0; h < VH; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int dim = 8 * (r + 8 * h) + 2 * j;
+        if (dim < D) {
+          float* d0 = &sm_o[warp][2 * c + 8 * t][dim];
+          float* d1 = &sm_o[warp][2 * c + 1 + 8 * t][dim];
+          *reinterpret_cast<float2*>(d0) = make_float2(o[4 * h + j][t][0], o[4 * h + j][t][2]);
+          *reinterpret_cast<float2*>(d1) = make_float2(o[4 * h + j][t][1], o[4 * h + j][t][3]);
+        }
+      }
+  }
+  __syncthreads();
+  if (tid < ROWS) {
+    float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kDecWarps; ++i) mm = fmaxf(mm, sm_m[i][tid]);
+#pragma unroll
+    for (int i = 0; i < kDecWarps; ++i) {
+      const float x = sm_m[i][tid], f = x == mm ? 1.0f : ex2t((x - mm) * cs);
+      sm_f[i][tid] = f;
+      ll = fmaf(sm_l[i][tid], f, ll);
+    }
+    sm_m[0][tid] = mm;
+    sm_l[0][tid] = ll;
+  }
+  __syncthreads();
+  for (int e = tid; e < ROWS * (D / 4); e += kDecThreads) {
+    const int i = e / (D / 4), d4 = e % (D / 4);
+    int b, head;
+    if (!row_of(i, b, head)) continue;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < kDecWarps; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(&sm_o[k][i][4 * d4]);
+      const float f = sm_f[k][i];
+      v.x = fmaf(x.x, f, v.x);
+      v.y = fmaf(x.y, f, v.y);
+      v.z = fmaf(x.z, f, v.z);
+      v.w = fmaf(x.w, f, v.w);
+    }
+    const float ll = sm_l[0][i];
+    if (p.parts == 1) {
+      const float inv = ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f;
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.o_stride_b + head * a.o_stride_h + 4 * d4) =
+          make_uint2(Half16<T>::pack(v.x * inv, v.y * inv), Half16<T>::pack(v.z * inv, v.w * inv));
+    } else {
+      const int64_t at = ((int64_t)b * a.q_heads + head) * p.parts + part;
+      if (d4 == 0) {
+        w.m[at] = sm_m[0][i] == -INFINITY ? -INFINITY : sm_m[0][i] * cs;
+        w.l[at] = ll;
+      }
+      if (ll != 0.0f) reinterpret_cast<float4*>(w.acc + at * D)[d4] = v;
     }
   }
+}
+
+// One warp per (sequence, head): the parts' sums, in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) decode_combine(const DecodeArgs a, int parts, const DecodeWs w) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= (int64_t)a.batch * a.q_heads) return;
+  const float *pm = w.m + row * parts, *pl = w.l + row * parts;
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32)
+    if (pl[i] != 0.0f) top = fmaxf(top, pm[i]);
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) from_f(own + a.prefix_len > 0 ? acc[i] / l : 0.0f, out + lane + 32 * i);
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float total = 0.0f;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    float f = 0.0f, lf = 0.0f;
+    if (i0 + lane < parts) {
+      const float x = pm[i0 + lane], li = pl[i0 + lane];
+      f = li == 0.0f ? 0.0f : (x == top ? 1.0f : ex2t(x - top));
+      lf = li == 0.0f ? 0.0f : li * f;
+    }
+    const uint32_t some = __ballot_sync(0xffffffffu, f != 0.0f || lf != lf);
+    for (int i = 0; i < 32 && i0 + i < parts; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      total += __shfl_sync(0xffffffffu, lf, i);
+      if (!(some >> i & 1u)) continue;  // a part without tokens wrote no sums
+      if (4 * lane < D) {
+        const float4 x = reinterpret_cast<const float4*>(w.acc + (row * parts + i0 + i) * D)[lane];
+        v.x = fmaf(x.x, fi, v.x);
+        v.y = fmaf(x.y, fi, v.y);
+        v.z = fmaf(x.z, fi, v.z);
+        v.w = fmaf(x.w, fi, v.w);
+      }
+    }
+  }
+  const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+  if (4 * lane < D) {
+    const int64_t b = row / a.q_heads, head = row % a.q_heads;
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.o_stride_b + head * a.o_stride_h + 4 * lane) =
+        make_uint2(Half16<T>::pack(v.x * inv, v.y * inv), Half16<T>::pack(v.z * inv, v.w * inv));
+  }
+}
+
+template <typename T, int D>
+cudaError_t prefix_tiles(const DecodeArgs& d, const DecodePlan& p, const DecodeWs& w, cudaStream_t s) {
+  TileArgs a;
+  std::memset(&a, 0, sizeof(a));
+  const int group = d.q_heads / d.heads, page = 1 << d.page_shift;
+  a.q_heads = d.q_heads; a.heads = d.heads; a.gp = group; a.tq = kTile / group; a.units = d.heads;
+  a.scale = d.scale; a.c = d.scale * kLog2e;
+  a.table = d.prefix_table; a.batch = d.batch; a.key_len = d.prefix_len; a.n_pages = d.n_pages;
+  a.page_shift = d.page_shift;
+  a.row_tiles = p.row_tiles; a.tiles_per_split = p.tiles_per_split; a.parts = p.parts;
+  a.ws_m = w.m; a.ws_l = w.l; a.ws_acc = w.acc;
+  CUtensorMap qm, km, vm;
+  const int type = Half16<T>::kType;
+  const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)d.q_heads, (cuuint64_t)d.batch};
+  const int64_t qs[2] = {d.q_stride_h, d.q_stride_b};
+  const cuuint32_t qb[3] = {64, (cuuint32_t)a.gp, (cuuint32_t)a.tq};
+  const cuuint64_t kd[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)d.heads, (cuuint64_t)d.n_pages};
+  const int64_t ks[3] = {D, (int64_t)page * D, (int64_t)d.heads * page * D};
+  const cuuint32_t kb[4] = {64, (cuuint32_t)page, 1, 1};
+  if (!tiles_map(&qm, d.q, type, 3, qd, qs, qb) || !tiles_map(&km, d.k_pages, type, 4, kd, ks, kb) ||
+      !tiles_map(&vm, d.v_pages, type, 4, kd, ks, kb))
+    return cudaErrorInvalidValue;
+  const int64_t ctas = (int64_t)a.units * p.row_tiles * p.tile_splits;
+  return p.tile_split_streams ? run_tiles<T, D, true, true>(qm, km, vm, a, ctas, s)
+                              : run_tiles<T, D, true, false>(qm, km, vm, a, ctas, s);
+}
+
+template <typename T, int D>
+cudaError_t decode_d(const DecodeArgs& a, const DecodePlan& p, void* ws, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.batch * a.q_heads;
+  DecodeWs w{nullptr, nullptr, nullptr};
+  if (needs_parts(p)) {
+    w.acc = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
+    w.m = w.acc + rows * p.parts * D;
+    w.l = w.m + rows * p.parts;
+  }
+  if (p.tile_splits) {
+    const cudaError_t e = prefix_tiles<T, D>(a, p, w, s);
+    if (e != cudaSuccess) return e;
+  }
+  const int64_t items = (int64_t)a.batch * a.heads * p.own_rt * p.own_splits + (int64_t)a.heads * p.pre_rt * p.pre_splits;
+  if (items > 0x7fffffff) return cudaErrorInvalidValue;
+  if (items > 0) {
+    if (p.rows == 8) decode_rows<T, D, 8><<<(unsigned)items, kDecThreads, 0, s>>>(a, p, w);
+    else decode_rows<T, D, 16><<<(unsigned)items, kDecThreads, 0, s>>>(a, p, w);
+  }
+  if (p.parts == 0 || needs_parts(p)) decode_combine<T, D><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a, p.parts, w);
+  return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t run_decode(const DecodeArgs& a, cudaStream_t s) {
-  const dim3 g(a.q_heads, a.batch);
-  if (a.head_dim == 128) decode_kernel<T, 128><<<g, 32, 0, s>>>(a);
-  else if (a.head_dim == 96) decode_kernel<T, 96><<<g, 32, 0, s>>>(a);
-  else decode_kernel<T, 64><<<g, 32, 0, s>>>(a);
-  return cudaGetLastError();
+cudaError_t decode_t(const DecodeArgs& a, const DecodePlan& p, void* ws, cudaStream_t s) {
+  if (a.head_dim == 128) return decode_d<T, 128>(a, p, ws, s);
+  if (a.head_dim == 96) return decode_d<T, 96>(a, p, ws, s);
+  return decode_d<T, 64>(a, p, ws, s);
 }
 
 }  // namespace
 
-size_t decode_workspace_bytes(const DecodeArgs&) { return 0; }
+cudaError_t decode_take_error(unsigned int* bits, cudaStream_t s) { return tiles_error(bits, s); }
 
-cudaError_t launch_decode(const DecodeArgs& a, int dtype, void*, cudaStream_t s) {
-  return dtype == NQ_F16 ? run_decode<__half>(a, s) : run_decode<__nv_bfloat16>(a, s);
+size_t decode_workspace_bytes(const DecodeArgs& a) {
+  const DecodePlan p = decode_plan(a);
+  if (!needs_parts(p)) return 0;
+  return (size_t)a.batch * a.q_heads * p.parts * (a.head_dim + 2) * sizeof(float) + 256;
+}
+
+cudaError_t launch_decode(const DecodeArgs& a, int dtype, void* ws, cudaStream_t s) {
+  const DecodePlan p = decode_plan(a);
+  return dtype == NQ_F16 ? decode_t<__half>(a, p, ws, s) : decode_t<__nv_bfloat16>(a, p, ws, s);
 }
 
 }  // namespace nq

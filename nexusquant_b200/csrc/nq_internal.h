@@ -198,6 +198,7 @@ struct DecodeArgs {
   int64_t q_stride_b, q_stride_h, o_stride_b, o_stride_h;
   float scale;
 };
+cudaError_t decode_take_error(unsigned int* bits, cudaStream_t s);  // read and clear its wait-error word
 size_t decode_workspace_bytes(const DecodeArgs& a);
 cudaError_t launch_decode(const DecodeArgs& a, int dtype, void* ws, cudaStream_t s);
 

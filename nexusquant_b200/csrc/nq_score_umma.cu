@@ -449,7 +449,9 @@ extern "C" nq_status_t nq_device_error(int32_t* bits, nq_stream_t stream) {
   if (nq::attend_take_error(&at, s) != cudaSuccess) return NQ_ERR_CUDA;
   if (at) v |= 4u;  // decode attention
   if (nq::prompt_take_error(&at, s) != cudaSuccess) return NQ_ERR_CUDA;
-  if (at) v |= 8u;  // attention over tiles
+  if (at) v |= 8u;  // prompt attention
+  if (nq::decode_take_error(&at, s) != cudaSuccess) return NQ_ERR_CUDA;
+  if (at) v |= 8u;  // shared prefix of the decode attention over pages
   if (bits) *bits = static_cast<int32_t>(v);
   return v ? NQ_ERR_TIMEOUT : NQ_OK;
 }
