@@ -21,11 +21,12 @@ constexpr int kDecWarps = 4;
 constexpr int kDecThreads = 32 * kDecWarps;
 constexpr int kGroup = 16;       // tokens per warp step
 constexpr int kMaxParts = 256;
+constexpr int kDecResident = 3;  // CTAs of decode_rows per SM
 
 struct DecodePlan {
   int rows;          // rows per CTA of decode_rows: 8 or 16
-  int own_rt, own_splits;
-  int pre_rt, pre_splits;      // prefix by decode_rows (0 splits: by attend_tiles or none)
+  int own_rt, own_splits, own_tokens;  // tokens per part, a multiple of 64
+  int pre_rt, pre_splits, pre_tokens;  // prefix by decode_rows (0 splits: by attend_tiles or none)
   int tile_splits, tiles_per_split, row_tiles;
   bool tile_split_streams;
   int parts;         // tile_splits + pre_splits + own_splits
@@ -40,17 +41,22 @@ DecodePlan decode_plan(const DecodeArgs& a) {
   const bool tiles = a.prefix_len > 0 && pre_rows > 16 && group <= kTile;
   p.rows = group <= 8 && (tiles || a.prefix_len == 0 || pre_rows <= 8) ? 8 : 16;
   p.own_rt = (group + p.rows - 1) / p.rows;
-  // CTAs of decode_rows resident at once; a part has at least one group per warp
-  const int64_t slots = 3ll * sms;
-  auto splits_for = [&](int64_t items, int tokens) {
-    const int most = (tokens + kGroup * kDecWarps - 1) / (kGroup * kDecWarps);
-    const int64_t want = std::max<int64_t>(1, slots / std::max<int64_t>(items, 1));
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, most), kMaxParts / 4));
+  // Parts of equal length, so that sequences of different lengths balance: enough of them for four
+  // rounds of the resident CTAs if all were as long as the bound, at least one step per warp.
+  const int64_t ctas = 4ll * kDecResident * sms;
+  auto tokens_for = [&](int64_t items, int tokens) {
+    const int64_t want = std::min<int64_t>(std::max<int64_t>(1, ctas / std::max<int64_t>(items, 1)), kMaxParts / 4);
+    const int step = kGroup * kDecWarps;
+    return (int)((((tokens + want - 1) / want) + step - 1) / step * step);
   };
-  if (a.max_len > 0) p.own_splits = splits_for((int64_t)a.batch * a.heads * p.own_rt, a.max_len);
+  if (a.max_len > 0) {
+    p.own_tokens = tokens_for((int64_t)a.batch * a.heads * p.own_rt, a.max_len);
+    p.own_splits = (a.max_len + p.own_tokens - 1) / p.own_tokens;
+  }
   if (a.prefix_len > 0 && !tiles) {
     p.pre_rt = (int)((pre_rows + p.rows - 1) / p.rows);
-    p.pre_splits = splits_for((int64_t)a.heads * p.pre_rt, a.prefix_len);
+    p.pre_tokens = tokens_for((int64_t)a.heads * p.pre_rt, a.prefix_len);
+    p.pre_splits = (a.prefix_len + p.pre_tokens - 1) / p.pre_tokens;
   }
   if (tiles) {
     const int tq = kTile / group, key_tiles = (a.prefix_len + kTile - 1) / kTile;
@@ -117,7 +123,7 @@ __device__ __forceinline__ uint4 ld_stream(const void* p) {
 //     2c + 8, 2c + 9) and interleaves them with byte permutes; the order of dimensions over the
 //     operand's rows is free.
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(kDecThreads, 3) decode_rows(const DecodeArgs a, const DecodePlan p, const DecodeWs w) {
+__global__ void __launch_bounds__(kDecThreads, kDecResident) decode_rows(const DecodeArgs a, const DecodePlan p, const DecodeWs w) {
   constexpr int KJ = D / 32;            // 16-byte chunks of a K row per lane
   constexpr int VH = (D + 63) / 64;     // of a V row
   constexpr int NT = ROWS / 8;          // column tiles of O^T
@@ -127,28 +133,30 @@ __global__ void __launch_bounds__(kDecThreads, 3) decode_rows(const DecodeArgs a
   const int group = a.q_heads / a.heads;
 
   // ---- which rows, which tokens
-  int item = blockIdx.x, n, kh, rt, seq = 0, split, splits, part;
+  int item = blockIdx.x, n, kh, rt, seq = 0, split, part, t_begin;
   const int32_t* table;
   const int own_items = a.batch * a.heads * p.own_rt * p.own_splits;
   const bool own = item < own_items;
   if (own) {
-    splits = p.own_splits;
-    split = item % splits; item /= splits;
+    split = item % p.own_splits; item /= p.own_splits;
     kh = item % a.heads; item /= a.heads;
     rt = item % p.own_rt;
     seq = item / p.own_rt;
     n = min(max(a.lens[seq], 0), a.max_len);
     table = a.tables + (int64_t)seq * a.width;
     part = p.tile_splits + p.pre_splits + split;
+    t_begin = split * p.own_tokens;
+    n = min(n, t_begin + p.own_tokens);
   } else {
     item -= own_items;
-    splits = p.pre_splits;
-    split = item % splits; item /= splits;
+    split = item % p.pre_splits; item /= p.pre_splits;
     kh = item % a.heads;
     rt = item / a.heads;
     n = a.prefix_len;
     table = a.prefix_table;
     part = p.tile_splits + split;
+    t_begin = split * p.pre_tokens;
+    n = min(n, t_begin + p.pre_tokens);
   }
   // row i of the CTA: its sequence and head, or none
   auto row_of = [&](int i, int& b, int& head) {
@@ -162,6 +170,12 @@ __global__ void __launch_bounds__(kDecThreads, 3) decode_rows(const DecodeArgs a
     head = kh * group + x % group;
     return b < a.batch;
   };
+
+  if (t_begin >= n && p.parts > 1) {  // no tokens here: the part counts for nothing
+    int b, head;
+    if (tid < ROWS && row_of(tid, b, head)) w.l[((int64_t)b * a.q_heads + head) * p.parts + part] = 0.0f;
+    return;
+  }
 
   uint4 q[NT][KJ];
 #pragma unroll
@@ -184,10 +198,8 @@ __global__ void __launch_bounds__(kDecThreads, 3) decode_rows(const DecodeArgs a
     for (int i = 0; i < VH * 4; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.0f;
   }
 
-  const int groups = (n + kGroup - 1) / kGroup, per = (groups + splits - 1) / splits;
-  const int g1 = min(groups, (split + 1) * per);
-  for (int g = split * per + warp; g < g1; g += kDecWarps) {
-    const int t0 = g * kGroup, page = min(max(__ldg(table + (t0 >> a.page_shift)), 0), a.n_pages - 1);
+  for (int t0 = t_begin + warp * kGroup; t0 < n; t0 += kGroup * kDecWarps) {
+    const int page = min(max(__ldg(table + (t0 >> a.page_shift)), 0), a.n_pages - 1);
     const int64_t base = ((((int64_t)page * a.heads + kh) << a.page_shift) + (t0 & ((1 << a.page_shift) - 1))) * D;
     const T* kp = static_cast<const T*>(a.k_pages) + base;
     const T* vp = static_cast<const T*>(a.v_pages) + base;
