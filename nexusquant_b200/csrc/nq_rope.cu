@@ -8,11 +8,16 @@
 // the values go either to dense outputs or to slot = page * page_size + offset of the pages.
 //
 // Bound by memory: every element is read and written once (2 bytes in, 2 bytes out at fp16).
-// Eight lanes (four at d = 64) share a row: lane i holds elements 8i..8i+7 of each half, so both
-// halves of a rotation pair are in one thread and the mean is three (two) shuffles.  A group
-// takes kRows heads of one token and one kind at once: their loads are all in flight before the
-// first is used, and the products of weights and rotation (w c, w s) are formed once for them:
+// Sixteen lanes (eight at d = 64) share a row: lane i holds elements 4i..4i+3 of each half, so both
+// halves of a rotation pair are in one thread and the mean is four (three) shuffles.  A group of
+// lanes takes kRows heads of one kind (queries, keys or values) of one token at once and forms the
+// products of weights and rotation once for them:
 //   z[i] = (x[i] (w c)[i] - x[i + d/2] (w' s)[i]) / rms,  with w' the second half's weights.
+// It keeps its heads and walks over the tokens, so that everything but the token's rows and its
+// table row is set up once; the next token's rows are in flight while this one's are computed.
+// 16384 tokens of 64 + 8 + 8 heads of 128, fp16: 119 us, 5.69 TB/s (0.88 of the measured copy rate).
+// One unit per thread group and launch measured 135 us (issue-bound: 19 instructions an element, now
+// 9); more CTAs of fewer registers spill (6 per SM: 180 us), fewer leave too little in flight (4: 139).
 #include <cstring>
 
 #include "../../include/nexusquant_b200.h"
@@ -22,173 +27,220 @@
 namespace nq {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
+constexpr int kRopeResident = 5;  // CTAs per SM
 constexpr int kRows = 4;  // heads of one token per lane group
 
 template <typename T>
-struct Vec8 {
-  uint4 u[sizeof(T) / 2];
+struct Vec4 {
+  uint32_t u[sizeof(T)];  // 4 elements
 };
 
-template <typename T>
-__device__ __forceinline__ Vec8<T> ld8(const T* p) {
-  Vec8<T> v;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) v.u[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+// ONCE: a row, read by nobody else; otherwise weights and table rows, which many threads read.
+// (Rows loaded and stored as streams: 127 -> 119 us at 16384 tokens of 64 + 16 heads of 128, fp16;
+// the loads alone gave nothing.)
+template <bool ONCE, typename T>
+__device__ __forceinline__ Vec4<T> ld4(const T* p) {
+  Vec4<T> v;
+  if constexpr (sizeof(T) == 2) {
+    const uint2* q = reinterpret_cast<const uint2*>(p);
+    const uint2 x = ONCE ? __ldcs(q) : __ldg(q);
+    v.u[0] = x.x; v.u[1] = x.y;
+  } else {
+    const uint4* q = reinterpret_cast<const uint4*>(p);
+    const uint4 x = ONCE ? __ldcs(q) : __ldg(q);
+    v.u[0] = x.x; v.u[1] = x.y; v.u[2] = x.z; v.u[3] = x.w;
+  }
   return v;
 }
 template <typename T>
-__device__ __forceinline__ void st8(T* p, const Vec8<T>& v) {
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = v.u[i];
+__device__ __forceinline__ void st4(T* p, const Vec4<T>& v) {
+  if constexpr (sizeof(T) == 2) __stcs(reinterpret_cast<uint2*>(p), make_uint2(v.u[0], v.u[1]));
+  else __stcs(reinterpret_cast<uint4*>(p), make_uint4(v.u[0], v.u[1], v.u[2], v.u[3]));
 }
 
-__device__ __forceinline__ void narrow8(const float* o, Vec8<__half>& v) {
-  __half2 h[4];
+__device__ __forceinline__ void widen4(const Vec4<__half>& v, float* o) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(o[2 * i], o[2 * i + 1]);
-  memcpy(&v, h, 16);
-}
-__device__ __forceinline__ void narrow8(const float* o, Vec8<__nv_bfloat16>& v) {
-  __nv_bfloat162 h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
-  memcpy(&v, h, 16);
-}
-__device__ __forceinline__ void narrow8(const float* o, Vec8<float>& v) { memcpy(&v, o, 32); }
-
-template <typename T>
-__device__ __forceinline__ void widen8(const Vec8<T>& v, float* o) {
-  load8(reinterpret_cast<const T*>(&v), o);
-}
-
-// 8 norm weights from element i of a vector in the tensors' type or fp32; ones without a vector
-template <typename T>
-__device__ __forceinline__ void weights8(const void* w, int f32, int i, float* o) {
-  if (!w) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = 1.0f;
-  } else if (f32) {
-    load8(static_cast<const float*>(w) + i, o);
-  } else {
-    widen8(ld8(static_cast<const T*>(w) + i), o);
+  for (int i = 0; i < 2; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v.u[i]));
+    o[2 * i] = f.x;
+    o[2 * i + 1] = f.y;
   }
+}
+__device__ __forceinline__ void widen4(const Vec4<__nv_bfloat16>& v, float* o) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v.u[i]));
+    o[2 * i] = f.x;
+    o[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void widen4(const Vec4<float>& v, float* o) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __uint_as_float(v.u[i]);
+}
+__device__ __forceinline__ void narrow4(const float* o, Vec4<__half>& v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const __half2 h = __floats2half2_rn(o[2 * i], o[2 * i + 1]);
+    v.u[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ void narrow4(const float* o, Vec4<__nv_bfloat16>& v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(o[2 * i], o[2 * i + 1]);
+    v.u[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ void narrow4(const float* o, Vec4<float>& v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v.u[i] = __float_as_uint(o[i]);
+}
+
+// 4 norm weights from element i of a vector in the tensors' type or fp32; ones without a vector
+template <typename T>
+__device__ __forceinline__ void weights4(const void* w, int f32, int i, float* o) {
+  if (!w) o[0] = o[1] = o[2] = o[3] = 1.0f;
+  else if (f32) widen4(ld4<false>(static_cast<const float*>(w) + i), o);
+  else widen4(ld4<false>(static_cast<const T*>(w) + i), o);
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const NormRopeArgs a) {
-  constexpr int LPR = D == 64 ? 4 : 8;  // lanes per row (two of eight idle at d = 96)
+__global__ void __launch_bounds__(kRopeThreads, sizeof(T) == 2 ? kRopeResident : 4)
+    norm_rope_kernel(const NormRopeArgs a, int token_step, int rounds) {
+  constexpr int LPR = D == 64 ? 8 : 16;  // lanes per row (four of sixteen idle at d = 96)
   constexpr int HALF = D / 2;
-  const int lane = threadIdx.x % LPR, e = lane * 8;
-  const int64_t unit = ((int64_t)blockIdx.x * kRopeThreads + threadIdx.x) / LPR;
+  const int lane = threadIdx.x % LPR, e = lane * 4;
+  const unsigned group = (blockIdx.x * (unsigned)kRopeThreads + threadIdx.x) / LPR;
   // units of a token: its queries, its keys, its values
-  const int uq = (a.q_heads + kRows - 1) / kRows, uk = (a.heads + kRows - 1) / kRows;
-  const int upt = uq + (a.v ? 2 : 1) * uk;
-  const int64_t t = unit / upt;
-  const int u = (int)(unit - t * upt);
+  const unsigned uq = (a.q_heads + kRows - 1) / kRows, uk = (a.heads + kRows - 1) / kRows;
+  const unsigned upt = uq + (a.v ? 2 : 1) * uk;
+  const unsigned t0 = group / upt, u = group - t0 * upt;
   const int kind = u < uq ? 0 : (u < uq + uk ? 1 : 2);  // queries, keys, values
-  const int h0 = (kind == 0 ? u : kind == 1 ? u - uq : u - uq - uk) * kRows;
-  const bool on = t < a.tokens && lane < HALF / 8;
-  const int n = on ? min(kRows, (kind == 0 ? a.q_heads : a.heads) - h0) : 0;
+  const int h0 = (int)(kind == 0 ? u : kind == 1 ? u - uq : u - uq - uk) * kRows;
+  const bool on = t0 < (unsigned)token_step && lane < HALF / 4;
+  const int n = min(kRows, (kind == 0 ? a.q_heads : a.heads) - h0);
 
-  const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + e +
-                 t * (kind == 0 ? a.q_stride_t : kind == 1 ? a.k_stride_t : a.v_stride_t);
   const int64_t step = kind == 0 ? a.q_stride_h : kind == 1 ? a.k_stride_h : a.v_stride_h;
-  Vec8<T> lo[kRows], hi[kRows];
-#pragma unroll
-  for (int i = 0; i < kRows; ++i)
-    if (i < n) {
-      lo[i] = ld8(src + (h0 + i) * step);
-      hi[i] = ld8(src + (h0 + i) * step + HALF);
-    }
-  // where the rows go
-  T* dst = nullptr;
-  int64_t dstep = 0;
-  if (n > 0) {
-    if (kind == 0) {
-      dst = static_cast<T*>(a.q_out) + t * a.qo_stride_t;
-      dstep = a.qo_stride_h;
-    } else if (!a.k_pages) {
-      dst = static_cast<T*>(a.k_out) + t * a.ko_stride_t;
-      dstep = a.ko_stride_h;
-    } else {
-      const int64_t slot = a.slots[t], page = slot >> a.page_shift, off = slot & ((1 << a.page_shift) - 1);
-      if (slot >= 0 && page < a.n_pages)
-        dst = static_cast<T*>(kind == 2 ? a.v_pages : a.k_pages) + (((page * a.heads) << a.page_shift) + off) * (int64_t)D;
-      dstep = (int64_t)D << a.page_shift;
-    }
-    if (dst) dst += e + h0 * dstep;
-  }
+  const int64_t tstep = kind == 0 ? a.q_stride_t : kind == 1 ? a.k_stride_t : a.v_stride_t;
+  const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + e + h0 * step;
+  const bool paged = kind > 0 && a.k_pages;
+  const int64_t dstep = kind == 0 ? a.qo_stride_h : paged ? (int64_t)D << a.page_shift : a.ko_stride_h;
+  const int64_t dtstep = kind == 0 ? a.qo_stride_t : a.ko_stride_t;
+  T* dst0 = static_cast<T*>(kind == 0 ? a.q_out : paged ? (kind == 2 ? a.v_pages : a.k_pages) : a.k_out) + e + h0 * dstep;
   const void* w = kind == 0 ? a.q_weight : a.k_weight;
   const bool norm = kind < 2 && w;
-  u64 lc[4], hs[4], hc[4], ls[4];  // (w c), (w' s), (w' c), (w s) of the 8 pairs, packed
-  if (kind < 2 && dst) {
-    const int pos = min(max(a.positions[t], 0), a.rope_rows - 1);
-    float c[8], s[8], wl[8], wh[8];
-    load8(a.rope_cos + (int64_t)pos * HALF + e, c);
-    load8(a.rope_sin + (int64_t)pos * HALF + e, s);
-    weights8<T>(w, a.weight_f32, e, wl);
-    weights8<T>(w, a.weight_f32, HALF + e, wh);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const u64 c2 = pk(c[2 * j], c[2 * j + 1]), s2 = pk(s[2 * j], s[2 * j + 1]);
-      const u64 l2 = pk(wl[2 * j], wl[2 * j + 1]), h2 = pk(wh[2 * j], wh[2 * j + 1]);
-      lc[j] = mul2(l2, c2);
-      hs[j] = mul2(h2, pk(-s[2 * j], -s[2 * j + 1]));
-      hc[j] = mul2(h2, c2);
-      ls[j] = mul2(l2, s2);
-    }
+  const bool any_norm = a.q_weight || a.k_weight;
+  float wl[4], wh[4];
+  if (on && kind < 2) {
+    weights4<T>(w, a.weight_f32, e, wl);
+    weights4<T>(w, a.weight_f32, HALF + e, wh);
   }
+
+  Vec4<T> nlo[kRows], nhi[kRows];  // rows of the next token
+  int npos = 0, nslot = -1;
+  auto fetch = [&](int64_t t) {
+    if (!on || t >= a.tokens) return;
+    const T* p = src + t * tstep;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    float x[16];
-    u64 sum2 = 0ull;
-    if (kind < 2 && i < n) {
-      widen8(lo[i], x);
-      widen8(hi[i], x + 8);
-      if (norm) {
+    for (int i = 0; i < kRows; ++i)
+      if (i < n) {
+        nlo[i] = ld4<true>(p + i * step);
+        nhi[i] = ld4<true>(p + i * step + HALF);
+      }
+    if (kind < 2) npos = __ldg(a.positions + t);
+    if (paged) nslot = __ldg(a.slots + t);
+  };
+  fetch(t0);
+  for (int round = 0; round < rounds; ++round) {  // the same count for all lanes: the shuffles need them
+    const int64_t t = (int64_t)round * token_step + t0;
+    Vec4<T> lo[kRows], hi[kRows];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum2 = fma2(pk(x[2 * j], x[2 * j + 1]), pk(x[2 * j], x[2 * j + 1]), sum2);
+    for (int i = 0; i < kRows; ++i) { lo[i] = nlo[i]; hi[i] = nhi[i]; }
+    T* dst = nullptr;
+    if (on && t < a.tokens) {
+      if (!paged) {
+        dst = dst0 + t * dtstep;
+      } else if (nslot >= 0 && (nslot >> a.page_shift) < a.n_pages) {
+        const int64_t page = nslot >> a.page_shift, off = nslot & ((1 << a.page_shift) - 1);
+        dst = dst0 + (((page * a.heads) << a.page_shift) + off) * D;
       }
     }
-    float inv = 1.0f;
-    if (a.q_weight || a.k_weight) {  // uniform: every lane of the warp takes the shuffles
-      float s0, s1;
-      upk(sum2, s0, s1);
-      float sum = s0 + s1;
+    u64 lc[2], hs[2], hc[2], ls[2];  // (w c), -(w' s), (w' c), (w s) of the 4 pairs, packed
+    if (kind < 2 && dst) {
+      const int pos = min(max(npos, 0), a.rope_rows - 1);
+      float c[4], s[4];
+      widen4(ld4<false>(a.rope_cos + (int64_t)pos * HALF + e), c);
+      widen4(ld4<false>(a.rope_sin + (int64_t)pos * HALF + e), s);
 #pragma unroll
-      for (int o = 1; o < LPR; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (norm) inv = 1.0f / sqrtf(__fmaf_rn(sum, 1.0f / D, a.eps));
-    }
-    if (i >= n || !dst) continue;
-    if (kind < 2) {
-      float y[16];
-      const u64 inv2 = pk(inv, inv);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u64 x0 = pk(x[2 * j], x[2 * j + 1]), x1 = pk(x[8 + 2 * j], x[9 + 2 * j]);
-        upk(mul2(fma2(x0, lc[j], mul2(x1, hs[j])), inv2), y[2 * j], y[2 * j + 1]);
-        upk(mul2(fma2(x1, hc[j], mul2(x0, ls[j])), inv2), y[8 + 2 * j], y[9 + 2 * j]);
+      for (int j = 0; j < 2; ++j) {
+        const u64 c2 = pk(c[2 * j], c[2 * j + 1]), s2 = pk(s[2 * j], s[2 * j + 1]);
+        const u64 l2 = pk(wl[2 * j], wl[2 * j + 1]), h2 = pk(wh[2 * j], wh[2 * j + 1]);
+        lc[j] = mul2(l2, c2);
+        hs[j] = mul2(h2, pk(-s[2 * j], -s[2 * j + 1]));
+        hc[j] = mul2(h2, c2);
+        ls[j] = mul2(l2, s2);
       }
-      narrow8(y, lo[i]);
-      narrow8(y + 8, hi[i]);
     }
-    st8(dst + i * dstep, lo[i]);
-    st8(dst + i * dstep + HALF, hi[i]);
+    fetch(t + token_step);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      float x[8], inv = 1.0f;
+      if (kind < 2) {
+        widen4(lo[i], x);
+        widen4(hi[i], x + 4);
+      }
+      if (any_norm) {
+        float sum = 0.0f;
+        if (norm && dst && i < n) {
+          u64 sum2 = 0ull;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum2 = fma2(pk(x[2 * j], x[2 * j + 1]), pk(x[2 * j], x[2 * j + 1]), sum2);
+          float s0, s1;
+          upk(sum2, s0, s1);
+          sum = s0 + s1;
+        }
+#pragma unroll
+        for (int o = 1; o < LPR; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (norm) inv = rsqrtf(__fmaf_rn(sum, 1.0f / D, a.eps));
+      }
+      if (i >= n || !dst) continue;
+      if (kind < 2) {
+        float y[8];
+        const u64 inv2 = pk(inv, inv);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const u64 x0 = pk(x[2 * j], x[2 * j + 1]), x1 = pk(x[4 + 2 * j], x[5 + 2 * j]);
+          upk(mul2(fma2(x0, lc[j], mul2(x1, hs[j])), inv2), y[2 * j], y[2 * j + 1]);
+          upk(mul2(fma2(x1, hc[j], mul2(x0, ls[j])), inv2), y[4 + 2 * j], y[5 + 2 * j]);
+        }
+        narrow4(y, lo[i]);
+        narrow4(y + 4, hi[i]);
+      }
+      st4(dst + i * dstep, lo[i]);
+      st4(dst + i * dstep + HALF, hi[i]);
+    }
   }
 }
 
 template <typename T>
 cudaError_t run_norm_rope(const NormRopeArgs& a, cudaStream_t s) {
-  const int64_t units = (int64_t)a.tokens * ((a.q_heads + kRows - 1) / kRows +
-                                             (a.v ? 2 : 1) * ((a.heads + kRows - 1) / kRows));
-  const int lpr = a.head_dim == 64 ? 4 : 8;
-  const int64_t blocks = (units * lpr + kRopeThreads - 1) / kRopeThreads;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int64_t upt = (a.q_heads + kRows - 1) / kRows + (a.v ? 2ll : 1ll) * ((a.heads + kRows - 1) / kRows);
+  const int lpr = a.head_dim == 64 ? 8 : 16;
+  // as many tokens at once as the resident CTAs hold, in equal rounds
+  const int64_t hold = (int64_t)sms * kRopeResident * (kRopeThreads / lpr);
+  const int64_t at_once = hold / upt > 0 ? hold / upt : 1;
+  const int64_t rounds = (a.tokens + at_once - 1) / at_once, token_step = (a.tokens + rounds - 1) / rounds;
+  const int64_t blocks = (token_step * upt * lpr + kRopeThreads - 1) / kRopeThreads;
+  if (blocks * kRopeThreads > 0x7fffffff) return cudaErrorInvalidValue;
   const unsigned g = (unsigned)blocks;
-  if (a.head_dim == 128) norm_rope_kernel<T, 128><<<g, kRopeThreads, 0, s>>>(a);
-  else if (a.head_dim == 96) norm_rope_kernel<T, 96><<<g, kRopeThreads, 0, s>>>(a);
-  else norm_rope_kernel<T, 64><<<g, kRopeThreads, 0, s>>>(a);
+  const int st = (int)token_step, r = (int)rounds;
+  if (a.head_dim == 128) norm_rope_kernel<T, 128><<<g, kRopeThreads, 0, s>>>(a, st, r);
+  else if (a.head_dim == 96) norm_rope_kernel<T, 96><<<g, kRopeThreads, 0, s>>>(a, st, r);
+  else norm_rope_kernel<T, 64><<<g, kRopeThreads, 0, s>>>(a, st, r);
   return cudaGetLastError();
 }
 
