@@ -75,37 +75,6 @@ class AttendParams(ctypes.Structure):
                 ("out_stride_h", c_i64)]
 
 
-class NormRopeParams(ctypes.Structure):
-    _fields_ = [("dtype", c_i32), ("tokens", c_i32), ("q_heads", c_i32), ("heads", c_i32), ("head_dim", c_i32),
-                ("q", c_vp), ("k", c_vp), ("v", c_vp), ("q_stride_t", c_i64), ("q_stride_h", c_i64),
-                ("k_stride_t", c_i64), ("k_stride_h", c_i64), ("v_stride_t", c_i64), ("v_stride_h", c_i64),
-                ("q_weight", c_vp), ("k_weight", c_vp), ("weight_f32", c_i32), ("eps", c_f32), ("positions", c_vp),
-                ("rope_cos", c_vp), ("rope_sin", c_vp), ("rope_rows", c_i32), ("q_out", c_vp), ("k_out", c_vp),
-                ("qo_stride_t", c_i64), ("qo_stride_h", c_i64), ("ko_stride_t", c_i64), ("ko_stride_h", c_i64),
-                ("k_pages", c_vp), ("v_pages", c_vp), ("n_pages", c_i32), ("page_size", c_i32), ("slots", c_vp)]
-
-
-class AttendPromptParams(ctypes.Structure):
-    _fields_ = [("dtype", c_i32), ("n_seqs", c_i32), ("q_tokens", c_i32), ("k_tokens", c_i32), ("q_heads", c_i32),
-                ("heads", c_i32), ("head_dim", c_i32), ("q", c_vp), ("k", c_vp), ("v", c_vp),
-                ("q_stride_t", c_i64), ("q_stride_h", c_i64), ("k_stride_t", c_i64), ("k_stride_h", c_i64),
-                ("v_stride_t", c_i64), ("v_stride_h", c_i64), ("seq_starts", c_vp), ("k_starts", c_vp),
-                ("scale", c_f32), ("out", c_vp), ("o_stride_t", c_i64), ("o_stride_h", c_i64), ("lse", c_vp)]
-
-
-class AttendPagesParams(ctypes.Structure):
-    _fields_ = [("dtype", c_i32), ("batch", c_i32), ("q_heads", c_i32), ("heads", c_i32), ("head_dim", c_i32),
-                ("n_pages", c_i32), ("page_size", c_i32), ("q", c_vp), ("q_stride_b", c_i64), ("q_stride_h", c_i64),
-                ("k_pages", c_vp), ("v_pages", c_vp), ("tables", c_vp), ("table_width", c_i32), ("lens", c_vp),
-                ("max_len", c_i32), ("prefix_table", c_vp), ("prefix_len", c_i32), ("scale", c_f32), ("out", c_vp),
-                ("o_stride_b", c_i64), ("o_stride_h", c_i64)]
-
-
-class Pool(ctypes.Structure):
-    _fields_ = [("k_pages", c_vp), ("v_pages", c_vp), ("layers", c_i32), ("n_pages", c_i32), ("heads", c_i32),
-                ("page_size", c_i32), ("row_bytes", c_i32)]
-
-
 # name -> (restype, argtypes)
 _PROTOS = {
     "nq_status_string": (ctypes.c_char_p, [c_i32]),
@@ -143,12 +112,13 @@ _PROTOS = {
     "nq_unpack_nibbles": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_vp]),
     "nq_merge_apply": (c_i32, [ctypes.POINTER(c_vp), c_i32, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_vp, c_vp,
                                c_i32, c_vp, c_vp, c_vp]),
-    "nq_norm_rope_qk": (c_i32, [ctypes.POINTER(NormRopeParams), c_vp]),
-    "nq_attend_prompt": (c_i32, [ctypes.POINTER(AttendPromptParams), c_vp]),
-    "nq_attend_pages_workspace_size": (c_size, [ctypes.POINTER(AttendPagesParams)]),
-    "nq_attend_pages": (c_i32, [ctypes.POINTER(AttendPagesParams), c_vp, c_size, c_vp]),
-    "nq_copy_pages": (c_i32, [ctypes.POINTER(Pool), c_vp, c_vp, c_i32, c_vp]),
-    "nq_compact_pages": (c_i32, [ctypes.POINTER(Pool), c_i32, c_vp, c_i32, c_vp, c_i64, c_vp, c_i32, c_vp, c_i32,
+    # parameter structs of the serving operators come packed, as bytes (kernels.py)
+    "nq_norm_rope_qk": (c_i32, [c_vp, c_vp]),
+    "nq_attend_prompt": (c_i32, [c_vp, c_vp]),
+    "nq_attend_pages_workspace_size": (c_size, [c_vp]),
+    "nq_attend_pages": (c_i32, [c_vp, c_vp, c_size, c_vp]),
+    "nq_copy_pages": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_vp]),
+    "nq_compact_pages": (c_i32, [c_vp, c_i32, c_vp, c_i32, c_vp, c_i64, c_vp, c_i32, c_vp, c_i32,
                                  c_vp]),
     "nq_device_error": (c_i32, [ctypes.POINTER(c_i32), c_vp]),
     "nq_wait_selftest": (c_i32, [ctypes.c_uint32, c_vp]),

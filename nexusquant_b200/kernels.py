@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Union
 
@@ -651,17 +652,32 @@ def attend_compressed(q: torch.Tensor, codes: LayerCodes, positions: torch.Tenso
 
 # ---------------------------------------------------------------------------
 # Serving operators around the cache: tensors are [tokens, heads, head_dim]
+#
+# A decoding step calls these for every layer, and at a few tokens the host's share is what a call
+# costs: parameters are packed with struct (the C structs of include/nexusquant_b200.h, native
+# alignment), and attributes of a tensor are read once.
 # ---------------------------------------------------------------------------
 PAGE_SIZES = (16, 32, 64, 128)
 _HEAD_DIMS = (64, 96, 128)
+_ATTEND_DTYPES = (torch.float16, torch.bfloat16)
+_NORM_ROPE = struct.Struct("@5i3P6q2Pif3Pi2P4q2P2iP").pack
+_ATTEND_PROMPT = struct.Struct("@7i3P6q2PfP2qP").pack
+_ATTEND_PAGES = struct.Struct("@7iP2q3PiPiPifP2q").pack
+_POOL = struct.Struct("@2P5i").pack
+_CUDA_ONLY = "nexusquant_b200 kernels need CUDA tensors (there is no CPU path)"
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t itself when its rows are 16-byte aligned, contiguous elements; else a contiguous copy."""
-    per = 16 // t.element_size()
-    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and not any(s % per for s in t.stride()[:-1]):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _rows16(t: torch.Tensor):
+    """(t, address, strides of the two outer dimensions) with 16-byte aligned rows of contiguous
+    elements; t is a contiguous copy where its rows are not."""
+    ptr, (s0, s1, s2) = t.data_ptr(), t.stride()
+    per = 15 // t.element_size()
+    if ptr & 15 or s2 != 1 or s0 & per or s1 & per:
+        t = t.clone(memory_format=torch.contiguous_format)
+        ptr, (s0, s1, _) = t.data_ptr(), t.stride()
+    return t, ptr, s0, s1
 
 
 def _int32(t: torch.Tensor, dev) -> torch.Tensor:
@@ -670,49 +686,58 @@ def _int32(t: torch.Tensor, dev) -> torch.Tensor:
     return t.to(device=dev, dtype=torch.int32).contiguous()
 
 
-def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], dtypes) -> None:
-    """q [n, hq, d], k / v [m, h, d] on one device, of one dtype, hq a multiple of h, d 64, 96 or 128."""
-    for t in (q, k, v):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError("nexusquant_b200 kernels need CUDA tensors (there is no CPU path)")
-        if t.dtype != q.dtype or t.device != q.device:
-            raise ValueError("queries, keys and values must share dtype and device")
-        if t.dim() != 3 or t.shape[2] != q.shape[2]:
-            raise ValueError("queries, keys and values must be [tokens, heads, head_dim] with one head_dim")
-    if q.dtype not in dtypes:
-        raise TypeError(f"unsupported dtype {q.dtype}")
-    if q.shape[2] not in _HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {_HEAD_DIMS} (got {q.shape[2]})")
-    if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"{q.shape[1]} query heads are not a multiple of {k.shape[1]} KV heads")
-    if v is not None and v.shape != k.shape:
-        raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)} differ")
+def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], dtypes):
+    """q [n, hq, d], k / v [m, h, d] on one device, of one dtype, hq a multiple of h, d 64, 96 or 128.
+    Returns the shapes of q and k."""
+    index, dt = q.get_device(), q.dtype
+    if index < 0 or k.get_device() < 0 or (v is not None and v.get_device() < 0):
+        raise RuntimeError(_CUDA_ONLY)
+    if k.dtype != dt or k.get_device() != index or (v is not None and (v.dtype != dt or v.get_device() != index)):
+        raise ValueError("queries, keys and values must share dtype and device")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or qs[2] != ks[2]:
+        raise ValueError("queries, keys and values must be [tokens, heads, head_dim] with one head_dim")
+    if dt not in dtypes:
+        raise TypeError(f"unsupported dtype {dt}")
+    if qs[2] not in _HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {_HEAD_DIMS} (got {qs[2]})")
+    if ks[1] == 0 or qs[1] == 0 or qs[1] % ks[1]:
+        raise ValueError(f"{qs[1]} query heads are not a multiple of {ks[1]} KV heads")
+    if v is not None and v.shape != ks:
+        raise ValueError(f"keys {tuple(ks)} and values {tuple(v.shape)} differ")
+    return qs, ks
 
 
-def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dims: int) -> None:
-    """Pages [(layers,) n_pages, heads, page_size, head_dim], contiguous, keys and values alike."""
-    if not k_pages.is_cuda or not v_pages.is_cuda:
-        raise RuntimeError("nexusquant_b200 kernels need CUDA tensors (there is no CPU path)")
-    if k_pages.dim() != dims or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype \
-            or k_pages.device != v_pages.device:
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dims: int):
+    """Pages [(layers,) n_pages, heads, page_size, head_dim], contiguous, keys and values alike.
+    Returns their shape."""
+    index, shape = k_pages.get_device(), k_pages.shape
+    if index < 0 or v_pages.get_device() < 0:
+        raise RuntimeError(_CUDA_ONLY)
+    if len(shape) != dims or shape != v_pages.shape or k_pages.dtype != v_pages.dtype or index != v_pages.get_device():
         raise ValueError("key and value pages must share shape, dtype and device")
     if not k_pages.is_contiguous() or not v_pages.is_contiguous():
         raise ValueError("pages must be contiguous")
     if k_pages.dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {k_pages.dtype}")
-    if k_pages.shape[-2] not in PAGE_SIZES:
-        raise ValueError(f"page size must be one of {PAGE_SIZES} (got {k_pages.shape[-2]})")
-    if k_pages.shape[-1] not in _HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {_HEAD_DIMS} (got {k_pages.shape[-1]})")
+    if shape[-2] not in PAGE_SIZES:
+        raise ValueError(f"page size must be one of {PAGE_SIZES} (got {shape[-2]})")
+    if shape[-1] not in _HEAD_DIMS:
+        raise ValueError(f"head_dim must be one of {_HEAD_DIMS} (got {shape[-1]})")
+    return shape
 
 
-def _check_out(out: torch.Tensor, like: torch.Tensor) -> None:
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+def _out(out: Optional[torch.Tensor], like: torch.Tensor, shape):
+    """(out, address, outer strides): a new tensor of the given shape, or the caller's, checked."""
+    if out is None:
+        out = torch.empty(shape, dtype=like.dtype, device=like.device)
+        return out, out.data_ptr(), shape[1] * shape[2], shape[2]
+    if out.shape != shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError("out must have the queries' shape, dtype and device")
-    if _rows16(out) is not out or any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+    same, ptr, s0, s1 = _rows16(out)
+    if same is not out or any(st == 0 and n > 1 for st, n in zip(out.stride(), shape)):
         raise ValueError("out needs 16-byte aligned rows of contiguous elements that do not overlap")
+    return out, ptr, s0, s1
 
 
 def _logit_scale(scale: Optional[float]) -> float:
@@ -724,13 +749,16 @@ def _logit_scale(scale: Optional[float]) -> float:
     return float(scale)
 
 
-def _launch(dev: torch.device, fn: str, *args) -> None:
-    """Call an entry point on ``dev``'s current stream, with ``dev`` current while it launches."""
-    if torch.cuda.current_device() == dev.index:
-        N.call(fn, *args, _stream(dev))
+def _launch(index: int, fn: str, *args) -> None:
+    """Call an entry point on device ``index``'s current stream, with that device current."""
+    entry = getattr(N.load(), fn)
+    if _raw_device() == index:
+        status = entry(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            N.call(fn, *args, _stream(dev))
+        with torch.cuda.device(index):
+            status = entry(*args, _raw_stream(index))
+    if status:
+        N.check(fn, status)
 
 
 def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *,
@@ -751,66 +779,58 @@ def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *,
     rope_rows : RoPE table rows to use when every position is known to be below it; None reads
                 positions.max() (a host synchronisation) to size the table.
     Returns (q_out, k_out); k_out is None with pages.  Computed in fp32, rounded once."""
-    _check_qkv(q, k, v, _DTYPES)
-    n, hq, d = q.shape
-    h = k.shape[1]
-    dev = q.device
-    if k.shape[0] != n or positions.numel() != n:
-        raise ValueError(f"{k.shape[0]} keys and {positions.numel()} positions for {n} queries")
-    paged = k_pages is not None or v_pages is not None
-    if paged:
+    (n, hq, d), (nk, h, _) = _check_qkv(q, k, v, _DTYPES)
+    dev, dt = q.device, q.dtype
+    if nk != n or positions.numel() != n:
+        raise ValueError(f"{nk} keys and {positions.numel()} positions for {n} queries")
+    ko = kos0 = kos1 = vp = vs0 = vs1 = kp = vpp = n_pages = page = slot_p = 0
+    if k_pages is not None or v_pages is not None:
         if k_pages is None or v_pages is None or v is None or slots is None:
             raise ValueError("storing into pages needs k_pages, v_pages, v and slots")
-        _check_pages(k_pages, v_pages, 4)
-        if k_pages.dtype != q.dtype or k_pages.device != dev or k_pages.shape[1] != h or k_pages.shape[3] != d:
+        n_pages, hp, page, dp = _check_pages(k_pages, v_pages, 4)
+        if k_pages.dtype != dt or k_pages.device != dev or hp != h or dp != d:
             raise ValueError("pages must have the keys' dtype, device, heads and head_dim")
         if slots.numel() != n:
             raise ValueError(f"{slots.numel()} slots for {n} tokens")
         slots = _int32(slots, dev)
+        v, vp, vs0, vs1 = _rows16(v)
+        k_out, kp, vpp, slot_p = None, k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr()
     elif slots is not None:
         raise ValueError("slots need pages")
-    w32 = 0
+    else:
+        k_out, ko, kos0, kos1 = _out(k_out, k, (n, h, d))
+    w32 = False
     for w in (q_weight, k_weight):
         if w is not None:
             if w.numel() != d or w.device != dev:
                 raise ValueError("norm weights must be [head_dim] on the queries' device")
-            w32 |= int(w.dtype != q.dtype)
+            w32 = w32 or w.dtype != dt
     if w32:
         q_weight, k_weight = (None if w is None else w.float() for w in (q_weight, k_weight))
-    q_weight, k_weight = (None if w is None else _rows16(w) for w in (q_weight, k_weight))
-    q, k = _rows16(q), _rows16(k)
+    wq = wk = 0
+    if q_weight is not None:
+        q_weight = _weight16(q_weight)
+        wq = q_weight.data_ptr()
+    if k_weight is not None:
+        k_weight = _weight16(k_weight)
+        wk = k_weight.data_ptr()
+    q, qp, qs0, qs1 = _rows16(q)
+    k, kptr, ks0, ks1 = _rows16(k)
     positions = _int32(positions, dev)
     if rope_rows is None:
         rope_rows = int(positions.max().item()) + 1 if n else 1
     cos, sin = TABLES.get(dev, d, rope_base, int(rope_rows), rope_scaling)
-    if q_out is None:
-        q_out = torch.empty((n, hq, d), dtype=q.dtype, device=dev)
-    else:
-        _check_out(q_out, q)
-    p = N.NormRopeParams()
-    if paged:
-        v = _rows16(v)
-        k_out = None
-        p.v, p.v_stride_t, p.v_stride_h = v.data_ptr(), v.stride(0), v.stride(1)
-        p.k_pages, p.v_pages, p.slots = k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr()
-        p.n_pages, p.page_size = k_pages.shape[0], k_pages.shape[2]
-    else:
-        if k_out is None:
-            k_out = torch.empty((n, h, d), dtype=q.dtype, device=dev)
-        else:
-            _check_out(k_out, k)
-        p.k_out, p.ko_stride_t, p.ko_stride_h = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
-    p.dtype, p.tokens, p.q_heads, p.heads, p.head_dim = _DTYPES[q.dtype], n, hq, h, d
-    p.q, p.q_stride_t, p.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
-    p.k, p.k_stride_t, p.k_stride_h = k.data_ptr(), k.stride(0), k.stride(1)
-    p.q_weight, p.k_weight, p.weight_f32, p.eps = _ptr(q_weight), _ptr(k_weight), int(w32 or q.dtype == torch.float32), eps
-    p.positions, p.rope_cos, p.rope_sin, p.rope_rows = positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    p.q_out, p.qo_stride_t, p.qo_stride_h = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
-    _launch(dev, "nq_norm_rope_qk", ctypes.byref(p))
+    q_out, qo, qos0, qos1 = _out(q_out, q, (n, hq, d))
+    _launch(dev.index, "nq_norm_rope_qk", _NORM_ROPE(
+        _DTYPES[dt], n, hq, h, d, qp, kptr, vp, qs0, qs1, ks0, ks1, vs0, vs1, wq, wk,
+        int(w32 or dt == torch.float32), eps, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        qo, ko, qos0, qos1, kos0, kos1, kp, vpp, n_pages, page, slot_p))
     return q_out, k_out
 
 
-_ATTEND_DTYPES = (torch.float16, torch.bfloat16)
+def _weight16(w: torch.Tensor) -> torch.Tensor:
+    """A norm weight of contiguous elements at a 16-byte boundary."""
+    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
 
 
 def attend_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: torch.Tensor, *,
@@ -825,35 +845,29 @@ def attend_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts:
                  a prompt); its last query stands at its last key.  None: the same as seq_starts.
     Returns [n, hq, d] (and, with return_lse, the fp32 log of the softmax sums [n, hq]).  A query that
     sees no key gets zeros and -inf; keys that a query does not see never reach its row."""
-    _check_qkv(q, k, v, _ATTEND_DTYPES)
-    n, hq, d = q.shape
-    dev = q.device
+    (n, hq, d), (m, h, _) = _check_qkv(q, k, v, _ATTEND_DTYPES)
+    dev, dt = q.device, q.dtype
     if seq_starts.dim() != 1 or seq_starts.numel() < 1:
         raise ValueError("seq_starts must be [n_seqs + 1]")
+    seq_starts = _int32(seq_starts, dev)
     if k_starts is None:
-        if k.shape[0] != n:
-            raise ValueError(f"{k.shape[0]} keys for {n} queries: give k_starts")
-        k_starts = seq_starts = _int32(seq_starts, dev)
+        if m != n:
+            raise ValueError(f"{m} keys for {n} queries: give k_starts")
+        k_starts = seq_starts
     else:
         if k_starts.shape != seq_starts.shape:
             raise ValueError("k_starts and seq_starts must have the same shape")
-        seq_starts, k_starts = _int32(seq_starts, dev), _int32(k_starts, dev)
-    q, k, v = (_rows16(t if all(t.stride()) else t.contiguous()) for t in (q, k, v))  # no broadcast rows
-    if out is None:
-        out = torch.empty((n, hq, d), dtype=q.dtype, device=dev)
-    else:
-        _check_out(out, q)
+        k_starts = _int32(k_starts, dev)
+    # the copies to shared memory go by strides: tensors broadcast over heads or tokens are written out
+    q, qp, qs0, qs1 = _rows16(q if all(q.stride()) else q.contiguous())
+    k, kp, ks0, ks1 = _rows16(k if all(k.stride()) else k.contiguous())
+    v, vp, vs0, vs1 = _rows16(v if all(v.stride()) else v.contiguous())
+    out, op, os0, os1 = _out(out, q, (n, hq, d))
     lse = torch.empty((n, hq), dtype=torch.float32, device=dev) if return_lse else None
-    p = N.AttendPromptParams()
-    p.dtype, p.n_seqs, p.q_tokens, p.k_tokens = _DTYPES[q.dtype], seq_starts.numel() - 1, n, k.shape[0]
-    p.q_heads, p.heads, p.head_dim = hq, k.shape[1], d
-    p.q, p.q_stride_t, p.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
-    p.k, p.k_stride_t, p.k_stride_h = k.data_ptr(), k.stride(0), k.stride(1)
-    p.v, p.v_stride_t, p.v_stride_h = v.data_ptr(), v.stride(0), v.stride(1)
-    p.seq_starts, p.k_starts = seq_starts.data_ptr(), k_starts.data_ptr()
-    p.scale = _logit_scale(scale)
-    p.out, p.o_stride_t, p.o_stride_h, p.lse = out.data_ptr(), out.stride(0), out.stride(1), _ptr(lse)
-    _launch(dev, "nq_attend_prompt", ctypes.byref(p))
+    _launch(dev.index, "nq_attend_prompt", _ATTEND_PROMPT(
+        _DTYPES[dt], seq_starts.numel() - 1, n, m, hq, h, d, qp, kp, vp, qs0, qs1, ks0, ks1, vs0, vs1,
+        seq_starts.data_ptr(), k_starts.data_ptr(), _logit_scale(scale), op, os0, os1,
+        0 if lse is None else lse.data_ptr()))
     return (out, lse) if return_lse else out
 
 
@@ -872,18 +886,17 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     Returns [b, hq, d]; a sequence without any token gets zeros."""
     if q.dim() != 3:
         raise ValueError("queries must be [batch, heads, head_dim]")
-    _check_pages(k_pages, v_pages, 4)
+    n_pages, h, page, dp = _check_pages(k_pages, v_pages, 4)
     b, hq, d = q.shape
-    n_pages, h, page, dp = k_pages.shape
-    if not q.is_cuda:
-        raise RuntimeError("nexusquant_b200 kernels need CUDA tensors (there is no CPU path)")
-    if q.dtype not in _ATTEND_DTYPES:
-        raise TypeError(f"unsupported dtype {q.dtype}")
-    if q.dtype != k_pages.dtype or q.device != k_pages.device or d != dp:
+    dev, dt = q.device, q.dtype
+    if q.get_device() < 0:
+        raise RuntimeError(_CUDA_ONLY)
+    if dt not in _ATTEND_DTYPES:
+        raise TypeError(f"unsupported dtype {dt}")
+    if dt != k_pages.dtype or q.get_device() != k_pages.get_device() or d != dp:
         raise ValueError("queries and pages must share dtype, device and head_dim")
     if h == 0 or hq == 0 or hq % h:
         raise ValueError(f"{hq} query heads are not a multiple of {h} KV heads")
-    dev = q.device
     if tables.dim() != 2 or tables.shape[0] != b or lens.numel() != b:
         raise ValueError(f"tables must be [{b}, width] and lens [{b}]")
     width = tables.shape[1]
@@ -891,38 +904,31 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
         max_len = width * page
     if not 0 <= max_len <= width * page:
         raise ValueError(f"max_len {max_len} outside the tables' {width * page} tokens")
-    if prefix_len < 0 or (prefix_len and (prefix_table is None or prefix_table.numel() * page < prefix_len)):
-        raise ValueError(f"prefix_table does not hold {prefix_len} tokens")
+    pre = 0
+    if prefix_len:
+        if prefix_len < 0 or prefix_table is None or prefix_table.numel() * page < prefix_len:
+            raise ValueError(f"prefix_table does not hold {prefix_len} tokens")
+        prefix_table = _int32(prefix_table, dev)
+        pre = prefix_table.data_ptr()
     tables, lens = _int32(tables, dev), _int32(lens, dev)
-    prefix_table = _int32(prefix_table, dev) if prefix_len else None
-    q = _rows16(q)
-    if out is None:
-        out = torch.empty((b, hq, d), dtype=q.dtype, device=dev)
-    else:
-        _check_out(out, q)
-    p = N.AttendPagesParams()
-    p.dtype, p.batch, p.q_heads, p.heads, p.head_dim = _DTYPES[q.dtype], b, hq, h, d
-    p.n_pages, p.page_size = n_pages, page
-    p.q, p.q_stride_b, p.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
-    p.k_pages, p.v_pages = k_pages.data_ptr(), v_pages.data_ptr()
-    p.tables, p.table_width, p.lens, p.max_len = tables.data_ptr(), width, lens.data_ptr(), int(max_len)
-    p.prefix_table, p.prefix_len = _ptr(prefix_table), int(prefix_len)
-    p.scale = _logit_scale(scale)
-    p.out, p.o_stride_b, p.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
-    ref = ctypes.byref(p)
-    nbytes = N.load().nq_attend_pages_workspace_size(ref)
+    q, qp, qs0, qs1 = _rows16(q if all(q.stride()) else q.contiguous())
+    out, op, os0, os1 = _out(out, q, (b, hq, d))
+    p = _ATTEND_PAGES(_DTYPES[dt], b, hq, h, d, n_pages, page, qp, qs0, qs1, k_pages.data_ptr(), v_pages.data_ptr(),
+                      tables.data_ptr(), width, lens.data_ptr(), max_len, pre, prefix_len, _logit_scale(scale), op, os0,
+                      os1)
+    nbytes = N.load().nq_attend_pages_workspace_size(p)
     # scratch from torch's allocator each call: it belongs to the current stream, captured or not
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _launch(dev, "nq_attend_pages", ref, _ptr(ws), nbytes)
+    _launch(dev.index, "nq_attend_pages", p, 0 if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
-def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor) -> N.Pool:
-    if k_pages.dim() == 4:
-        k_pages, v_pages = k_pages.unsqueeze(0), v_pages.unsqueeze(0)
-    _check_pages(k_pages, v_pages, 5)
-    layers, n_pages, h, page, d = k_pages.shape
-    return N.Pool(k_pages.data_ptr(), v_pages.data_ptr(), layers, n_pages, h, page, d * k_pages.element_size())
+def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor):
+    """(packed nq_pool_t, pages, page size) of [layers, ...] pages or of one layer's."""
+    shape = _check_pages(k_pages, v_pages, 4 if k_pages.dim() == 4 else 5)
+    layers, (n_pages, h, page, d) = (1 if len(shape) == 4 else shape[0]), shape[-4:]
+    return (_POOL(k_pages.data_ptr(), v_pages.data_ptr(), layers, n_pages, h, page, d * k_pages.element_size()),
+            n_pages, page)
 
 
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -931,18 +937,18 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     k_pages, v_pages : [layers, n_pages, h, page_size, d] (or one layer's 4-D pages).
     src, dst         : int32 [n].  No page of dst may be in src or twice in dst: pairs given on
                        the CPU are checked, those on the device are taken as they are."""
-    pool = _pool(k_pages, v_pages)
+    pool, n_pages, _ = _pool(k_pages, v_pages)
     if src.shape != dst.shape or src.dim() != 1:
         raise ValueError("src and dst must be [n]")
     if not src.is_cuda and not dst.is_cuda:
         s, t = src.tolist(), dst.tolist()
         if len(set(t)) < len(t) or set(s) & set(t):
             raise ValueError("a destination page is also a source or is written twice")
-        if s and not (0 <= min(s + t) and max(s + t) < pool.n_pages):
-            raise ValueError(f"page numbers outside the pool of {pool.n_pages}")
+        if s and not (0 <= min(s + t) and max(s + t) < n_pages):
+            raise ValueError(f"page numbers outside the pool of {n_pages}")
     dev = k_pages.device
     src, dst = _int32(src, dev), _int32(dst, dev)
-    _launch(dev, "nq_copy_pages", ctypes.byref(pool), src.data_ptr(), dst.data_ptr(), src.numel())
+    _launch(dev.index, "nq_copy_pages", pool, src.data_ptr(), dst.data_ptr(), src.numel())
 
 
 def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, kept_idx: torch.Tensor,
@@ -956,13 +962,13 @@ def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Te
     kept_idx, kept_count : as select_keep returns them (int32 [b, T] ascending, [b]); None: max_kept each.
     max_kept             : bound on kept_count (a host number); None: what kept_idx and the fresh pages
                            can hold."""
-    pool = _pool(k_pages, v_pages)
+    pool, _, page = _pool(k_pages, v_pages)
     if tables.dim() != 2 or dst_tables.dim() != 2 or kept_idx.dim() != 2:
         raise ValueError("tables, dst_tables and kept_idx must be [batch, ...]")
     b = tables.shape[0]
     if dst_tables.shape[0] != b or kept_idx.shape[0] != b or (kept_count is not None and kept_count.numel() != b):
         raise ValueError(f"dst_tables, kept_idx and kept_count must have {b} rows")
-    holds = min(kept_idx.shape[1], dst_tables.shape[1] * pool.page_size)
+    holds = min(kept_idx.shape[1], dst_tables.shape[1] * page)
     if max_kept is None:
         max_kept = holds
     if not 0 <= max_kept <= holds:
@@ -970,5 +976,6 @@ def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Te
     dev = k_pages.device
     tables, dst_tables, kept_idx = _int32(tables, dev), _int32(dst_tables, dev), _int32(kept_idx, dev)
     kept_count = None if kept_count is None else _int32(kept_count, dev)
-    _launch(dev, "nq_compact_pages", ctypes.byref(pool), b, tables.data_ptr(), tables.shape[1], kept_idx.data_ptr(),
-            kept_idx.shape[1], _ptr(kept_count), int(max_kept), dst_tables.data_ptr(), dst_tables.shape[1])
+    _launch(dev.index, "nq_compact_pages", pool, b, tables.data_ptr(), tables.shape[1], kept_idx.data_ptr(),
+            kept_idx.shape[1], 0 if kept_count is None else kept_count.data_ptr(),
+            int(max_kept), dst_tables.data_ptr(), dst_tables.shape[1])

@@ -656,53 +656,56 @@ def test_refusals():
             pytest.fail(f"case {i} was not refused")
 
 
+# fields of the C parameter structs, in order (include/nexusquant_b200.h)
+ROPE_FIELDS = """dtype tokens q_heads heads head_dim q k v q_stride_t q_stride_h k_stride_t k_stride_h v_stride_t v_stride_h
+    q_weight k_weight weight_f32 eps positions rope_cos rope_sin rope_rows q_out k_out qo_stride_t qo_stride_h ko_stride_t
+    ko_stride_h k_pages v_pages n_pages page_size slots""".split()
+PROMPT_FIELDS = """dtype n_seqs q_tokens k_tokens q_heads heads head_dim q k v q_stride_t q_stride_h k_stride_t k_stride_h
+    v_stride_t v_stride_h seq_starts k_starts scale out o_stride_t o_stride_h lse""".split()
+PAGES_FIELDS = """dtype batch q_heads heads head_dim n_pages page_size q q_stride_b q_stride_h k_pages v_pages tables
+    table_width lens max_len prefix_table prefix_len scale out o_stride_b o_stride_h""".split()
+
+
 def test_entry_points_refuse_without_a_gpu():
     """Host checks of the C entry points; each returns before anything is launched."""
-    import ctypes
     lib = N.load()
     one = 4096  # an aligned, never used address
 
-    def rope(**kw):
-        p = N.NormRopeParams(dtype=0, tokens=2, q_heads=4, heads=2, head_dim=128, q=one, k=one, q_out=one, k_out=one,
-                             positions=one, rope_cos=one, rope_sin=one, rope_rows=8)
-        for n, v in kw.items():
-            setattr(p, n, v)
-        return lib.nq_norm_rope_qk(ctypes.byref(p), None)
+    def maker(fields, pack, call, **base):
+        def run(**kw):
+            assert set(kw) <= set(fields)
+            return call(pack(*[{**base, **kw}.get(f, 0) for f in fields]))
+        return run
 
+    rope = maker(ROPE_FIELDS, K._NORM_ROPE, lambda p: lib.nq_norm_rope_qk(p, None), dtype=0, tokens=2, q_heads=4, heads=2,
+                 head_dim=128, q=one, k=one, q_out=one, k_out=one, positions=one, rope_cos=one, rope_sin=one, rope_rows=8)
     assert lib.nq_norm_rope_qk(None, None) == -1
     assert rope(tokens=0) == 0 and rope(tokens=-1) == -1 and rope(head_dim=80) == -2 and rope(dtype=3) == -1
-    assert rope(k_out=None) == -1 and rope(rope_rows=0) == -1 and rope(q=one + 8) == -6 and rope(q_stride_t=4) == -6
+    assert rope(k_out=0) == -1 and rope(rope_rows=0) == -1 and rope(q=one + 8) == -6 and rope(q_stride_t=4) == -6
     assert rope(k_pages=one) == -1 and rope(k_pages=one, v_pages=one, page_size=48) == -2
     assert rope(k_pages=one, v_pages=one, page_size=16) == -1  # no v, no slots
 
-    def prompt(**kw):
-        p = N.AttendPromptParams(dtype=0, n_seqs=1, q_tokens=2, k_tokens=2, q_heads=4, heads=2, head_dim=128, q=one, k=one,
-                                 v=one, seq_starts=one, k_starts=one, out=one)
-        for n, v in kw.items():
-            setattr(p, n, v)
-        return lib.nq_attend_prompt(ctypes.byref(p), None)
-
+    prompt = maker(PROMPT_FIELDS, K._ATTEND_PROMPT, lambda p: lib.nq_attend_prompt(p, None), dtype=0, n_seqs=1, q_tokens=2,
+                   k_tokens=2, q_heads=4, heads=2, head_dim=128, q=one, k=one, v=one, seq_starts=one, k_starts=one, out=one)
     assert lib.nq_attend_prompt(None, None) == -1
     assert prompt(q_tokens=0) == 0 and prompt(n_seqs=0) == 0 and prompt(dtype=2) == -2 and prompt(head_dim=32) == -2
-    assert prompt(q_heads=3) == -2 and prompt(out=None) == -1 and prompt(seq_starts=None) == -1
+    assert prompt(q_heads=3) == -2 and prompt(out=0) == -1 and prompt(seq_starts=0) == -1 and prompt(scale=-0.5) == -1
     assert prompt(v=one + 2) == -6 and prompt(k_stride_h=12) == -6
 
-    def pages(**kw):
-        p = N.AttendPagesParams(dtype=0, batch=1, q_heads=4, heads=2, head_dim=128, n_pages=4, page_size=16, q=one,
-                                k_pages=one, v_pages=one, tables=one, table_width=2, lens=one, max_len=32, out=one)
-        for n, v in kw.items():
-            setattr(p, n, v)
-        return lib.nq_attend_pages(ctypes.byref(p), None, 0, None)
-
+    pages = maker(PAGES_FIELDS, K._ATTEND_PAGES, lambda p: lib.nq_attend_pages(p, None, 0, None), dtype=0, batch=1,
+                  q_heads=4, heads=2, head_dim=128, n_pages=4, page_size=16, q=one, k_pages=one, v_pages=one, tables=one,
+                  table_width=2, lens=one, max_len=32, out=one)
     assert lib.nq_attend_pages(None, None, 0, None) == -1 and lib.nq_attend_pages_workspace_size(None) == 0
     assert pages(batch=0) == 0 and pages(page_size=8) == -2 and pages(max_len=33) == -1 and pages(n_pages=0) == -1
-    assert pages(prefix_len=4) == -1 and pages(q=None) == -1 and pages(out=one + 4) == -6 and pages(dtype=2) == -2
-    pool = N.Pool(one, one, 2, 4, 2, 16, 256)
-    assert lib.nq_copy_pages(None, one, one, 1, None) == -1 and lib.nq_copy_pages(ctypes.byref(pool), one, one, 0, None) == 0
-    assert lib.nq_copy_pages(ctypes.byref(pool), None, one, 1, None) == -1
-    assert lib.nq_compact_pages(ctypes.byref(pool), 1, one, 2, one, 32, None, 17, one, 1, None) == -1
-    assert lib.nq_compact_pages(ctypes.byref(pool), 1, one, 2, one, 32, None, 0, one, 1, None) == 0
-    pool.row_bytes = 24
-    assert lib.nq_copy_pages(ctypes.byref(pool), one, one, 1, None) == -6
-    pool.page_size = 20
-    assert lib.nq_copy_pages(ctypes.byref(pool), one, one, 1, None) == -2
+    assert pages(prefix_len=4) == -1 and pages(q=0) == -1 and pages(out=one + 4) == -6 and pages(dtype=2) == -2
+    assert pages(max_len=32, batch=4096, scale=math.inf) == -1
+
+    def pool(page=16, row=256):
+        return K._POOL(one, one, 2, 4, 2, page, row)
+
+    assert lib.nq_copy_pages(None, one, one, 1, None) == -1 and lib.nq_copy_pages(pool(), one, one, 0, None) == 0
+    assert lib.nq_copy_pages(pool(), None, one, 1, None) == -1
+    assert lib.nq_compact_pages(pool(), 1, one, 2, one, 32, None, 17, one, 1, None) == -1
+    assert lib.nq_compact_pages(pool(), 1, one, 2, one, 32, None, 0, one, 1, None) == 0
+    assert lib.nq_copy_pages(pool(row=24), one, one, 1, None) == -6
+    assert lib.nq_copy_pages(pool(page=20), one, one, 1, None) == -2
