@@ -65,6 +65,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, kTileWait));
 }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
                                             uint32_t accumulate) {
   asm volatile(
@@ -256,7 +263,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tb = tmem_base;  // S (and P): columns 0, 128; O: columns 256, 384
+  const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0);  // S (and P): columns 0, 128; O: columns 256, 384
 
   // ---- key tiles of each stream: tile0 + u (SPLIT: tile0 + 2u + s), u < steps[s]
   int tile0 = 0, steps[2], lim_last;
@@ -276,6 +283,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       steps[1] = job.tokens > a.tq ? n : 0;
     }
   }
+  steps[0] = __shfl_sync(0xffffffffu, steps[0], 0);  // the same in all threads: keep loops on them uniform
+  steps[1] = __shfl_sync(0xffffffffu, steps[1], 0);
   const int all = max(steps[0], steps[1]);
   const int lim_first = PAGED ? job.klen - 1 : job.lim0;
   auto tile_of = [&](int u, int s) { return SPLIT ? tile0 + 2 * u + s : tile0 + u; };
@@ -287,10 +296,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // whether this use takes the item from the ring, and whether it is the last use of it.
   auto walk = [&](auto&& visit) {
     if (all == 0) return;
+#pragma unroll
     for (int s = 0; s < 2; ++s)
       if (steps[s] > 0 && !visit(0, 0, s, SPLIT || s == 0 || steps[0] == 0, SPLIT || s == 1 || steps[1] == 0)) return;
     for (int u = 0; u < all; ++u)
+#pragma unroll
       for (int s = 0; s < 2; ++s)
+#pragma unroll
         for (int kind = 1; kind >= 0; --kind) {
           const int w = kind ? u : u + 1;
           if (w >= steps[s]) continue;
@@ -354,47 +366,56 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
    } else if (warp == 9) {
     // -------------------------------------------------------------- products
-    if (lane == 0 && all > 0) {
+    // The whole warp runs this loop, converged, with one elected lane around the instructions: their
+    // descriptors then stay in uniform registers.  Issued by one lane of a divergent warp the same
+    // 4 x 8 products took 3400 cycles a step instead of 2190 (2050 is the tensor cores' own time).
+    if (all > 0) {
       constexpr uint32_t kIdS = f16_idesc(H::kType, kTile, kTile);
       constexpr uint32_t kIdO = f16_idesc(H::kType, kTile, D) | (1u << 16);  // B (values) MN-major
-      int it = 0, raw = 0;
-      bool ok = mbar_wait(&qfull, 0, kTileWait);
+      // descriptors without the address: K-major, and MN-major with the column blocks kBlock apart
+      constexpr uint64_t kDescK = (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+      constexpr uint64_t kDescV = ((uint64_t)(Lo::kBlock >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+      const uint32_t q16 = __shfl_sync(0xffffffffu, smem_u32(sm) >> 4, 0), ring16 = q16 + Lo::kQ / 16;
+      int slot = 0, raw = 0;
+      uint32_t round = 0;
       int slot_of[2] = {0, 0};  // where the K / V item in use lies
+      bool ok = warp_wait(&qfull, 0);
       if (ok)
         walk([&](int kind, int u, int s, bool first, bool last) {
-          if (kind == 1 && !mbar_wait(&pready[s], u & 1, kTileWait)) return ok = false;
           if (first) {
-            slot_of[kind] = it % NST;
-            if (!mbar_wait(&full[it % NST], (it / NST) & 1, kTileWait)) return ok = false;
-            ++it;
-            if (kind == 1 && hidden_keys(tile_of(u, s)) && !mbar_wait(&scrubbed[raw++ & 3], 0, kTileWait))
-              return ok = false;
+            slot_of[kind] = slot;
+            if (!warp_wait(&full[slot], round)) return ok = false;
+            if (++slot == NST) { slot = 0; round ^= 1u; }
+            if (kind == 1 && hidden_keys(tile_of(u, s)) && !warp_wait(&scrubbed[raw++ & 3], 0)) return ok = false;
           }
+          if (kind == 1 && !warp_wait(&pready[s], u & 1)) return ok = false;
           tc_fence_after();
-          const uint8_t* item = ring + slot_of[kind] * Lo::kItem;
-          if (kind == 0) {
-            const uint8_t* qs = sm + (SPLIT ? 0 : s * Lo::kItem);
+          const uint32_t item16 = ring16 + slot_of[kind] * (Lo::kItem / 16);
+          if (elect_one()) {
+            if (kind == 0) {
+              const uint32_t qs16 = q16 + (SPLIT ? 0 : s * (Lo::kItem / 16));
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const int off = (k >> 2) * Lo::kBlock + (k & 3) * 32;
-              umma_f16(tb + s * 128, sw128_desc(qs + off), sw128_desc(item + off), kIdS, k > 0 ? 1u : 0u);
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (k >> 2) * (Lo::kBlock / 16) + (k & 3) * 2;
+                umma_f16(tb + s * 128, kDescK | (qs16 + off), kDescK | (item16 + off), kIdS, k > 0 ? 1u : 0u);
+              }
+              umma_commit(&sfull[s]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < kTile / 16; ++k)
+                umma_f16_ts(tb + 256 + s * 128, tb + s * 128 + k * 8, kDescV | (item16 + k * 128), kIdO, u > 0 || k > 0 ? 1u : 0u);
+              if (u == steps[s] - 1) umma_commit(&odone[s]);
             }
-            umma_commit(&sfull[s]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              umma_f16_ts(tb + 256 + s * 128, tb + s * 128 + k * 8, sw128_mn_desc(item + k * 2048, Lo::kBlock, 1024), kIdO,
-                          u > 0 || k > 0 ? 1u : 0u);
-            if (u == steps[s] - 1) umma_commit(&odone[s]);
+            if (last) umma_commit(&empty[slot_of[kind]]);
           }
-          if (last) umma_commit(&empty[slot_of[kind]]);
+          __syncwarp();
           return true;
         });
       if (!ok) {
         err = 1;
         // products in flight end before the tensor memory is given up
-        umma_commit(&drain);
-        mbar_wait(&drain, 0, kTileWait);
+        if (elect_one()) umma_commit(&drain);
+        warp_wait(&drain, 0);
       }
     }
    } else {
