@@ -36,9 +36,14 @@ cudaError_t prompt_d(const PromptArgs& p, cudaStream_t s) {
   if (!tiles_map(&vm, keys ? p.v : p.q, type, 3, kd, keys ? vs : qs, kb)) return cudaErrorInvalidValue;
   // at most this many tiles of a CTA's tokens: one partly filled tile per sequence
   auto ctas = [&](int tok) { return ((int64_t)p.q_tokens / tok + p.n_seqs) * a.units; };
-  // two row tiles per CTA share their key tiles; a grid that does not fill the GPU that way takes
-  // one row tile per CTA, with its keys split between the streams
-  if (ctas(2 * a.tq) >= device_sms()) return run_tiles<T, D, false, false>(qm, km, vm, a, ctas(2 * a.tq), s);
+  // Two row tiles per job share their key tiles.  With one row tile per job, its keys split between
+  // the streams, a job takes half as long: better where that fills the last round of jobs.
+  const int sms = device_sms();
+  auto rounds = [&](int tok) {  // expected: a sequence's last tile is half empty on average
+    const int64_t jobs = ((int64_t)p.q_tokens / tok + (p.n_seqs + 1) / 2) * a.units;
+    return (double)((jobs + sms - 1) / sms);
+  };
+  if (2.0 * rounds(2 * a.tq) <= rounds(a.tq)) return run_tiles<T, D, false, false>(qm, km, vm, a, ctas(2 * a.tq), s);
   return run_tiles<T, D, false, true>(qm, km, vm, a, ctas(a.tq), s);
 }
 

@@ -12,12 +12,17 @@
 // grouped-query model fills the 128 rows from few tokens.  A CTA runs two such streams, each with
 // its own softmax warpgroup, so that the exponentials of one overlap the products of the other:
 //   SPLIT = false: stream s takes row tile s, both read the same key tiles;
-//   SPLIT = true : both take the same row tile, stream s the key tiles of parity s, merged at the
-//                  end in shared memory (for grids that would not fill the GPU).
+//   SPLIT = true : both take the same row tile, stream s the key tiles of parity s, joined at the
+//                  end (for grids that would not fill the GPU).
 // Warps 0-3 / 4-7: softmax of stream 0 / 1, one thread per row (TMEM lane).  Warp 8: TMA loads of
 // Q, K and V (128-byte swizzle) into a ring.  Warp 9: the MMAs: S = Q K^T from shared memory into
 // TMEM, O += P V with P read from TMEM (it overwrites S) and V as MN-major operand.  Warps 10-11:
-// clear the rows of V that no row of the CTA may see, see scrub().
+// keep values that a row may not see out of the products (below).
+//
+// A CTA stays and takes further jobs (row tiles x key range x KV head): it cancels the launch of a
+// CTA that has not started and does that one's work (cluster launch control), so the hardware's
+// order of the grid is kept.  The next job's Q, K and V are loaded, and its first S computed, while
+// the softmax warps still write the last one's rows.
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -158,20 +163,68 @@ struct TileLayout {
   static constexpr int kBlock = kTile * 128;             // one column block of a tile
   static constexpr int kItem = kBlocks * kBlock;         // a K, V or Q tile
   static constexpr int kQ = (SPLIT ? 1 : 2) * kItem;
-  static constexpr int kStages = (225 * 1024 - kQ) / kItem < 8 ? (225 * 1024 - kQ) / kItem : 8;
-  static constexpr int kMerge = SPLIT ? kTile * D * 4 + kTile * 8 : 0;  // stream 1's result, over the ring
-  static constexpr int kBytes = kQ + kStages * kItem + 1024;
-  static_assert(kMerge <= kStages * kItem, "the merge buffer lies in the ring");
+  static constexpr int kStages = (224 * 1024 - kQ) / kItem < 8 ? (224 * 1024 - kQ) / kItem : 8;
+  static constexpr int kMl = SPLIT ? 2 * kTile * 8 : 0;  // (m, l) of each row and stream
+  static constexpr int kBytes = kQ + kStages * kItem + kMl;
+  // with the barriers (under 1 KB, and the tiles start at a multiple of that) at most 227 KB
+  static_assert(kBytes + 1024 <= 227 * 1024, "shared memory of a CTA");
 };
 
-// Where a CTA works: rows q0 .. q0 + tokens of q (gp heads each), keys k0 .. k0 + klen, and the last
-// key that its first token sees (each further token sees one more).
+// A CTA's work: rows q0 .. q0 + tokens of q (gp heads each), keys k0 .. k0 + klen, the last key that
+// its first token sees (each further token sees one more); tokens = 0: nothing, -1: no more jobs.
 struct TileJob {
-  int q0, tokens, k0, klen, lim0;
+  int q0, tokens, k0, klen, lim0, unit, split;
+};
+
+// The key tiles of a job: stream s takes tile0 + u (SPLIT: tile0 + 2u + s) for u < steps[s].
+struct TileSpan {
+  int tile0, steps[2], all, lim_first, lim_last;
 };
 
 // Device error word of the bounded waits below (bit 8 of nq_device_error), one per including file.
 __device__ unsigned int g_tiles_wait_error;
+
+// The next job's grid index, or -1 when every CTA of the grid has started: issue, and the answer.
+__device__ __forceinline__ void clc_ask(uint4* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ int clc_answer(const uint4* answer) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\tmov.b32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, r;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return ok ? (int)x : -1;
+}
+
+// 4 x 4 units of 16 bytes between the four lanes of a quad: afterwards unit j of lane i is unit i of
+// lane j, so that four lanes store 64 consecutive bytes of one row.
+__device__ __forceinline__ void quad_transpose(uint32_t (&w)[16], int lane) {
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j & o) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t send = up ? w[4 * j + e] : w[4 * (j + o) + e];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, send, o);
+        if (up) w[4 * j + e] = got;
+        else w[4 * (j + o) + e] = got;
+      }
+    }
+  }
+}
 
 template <typename T, int D, bool PAGED, bool SPLIT>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -180,188 +233,254 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   using Lo = TileLayout<D, SPLIT>;
   using H = Half16<T>;
   constexpr int NST = Lo::kStages;
-  extern __shared__ uint8_t tiles_smem_raw[];
-  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tiles_smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t sm[];  // the 128-byte swizzle counts from multiples of 1024
   uint8_t* ring = sm + Lo::kQ;
-  __shared__ uint64_t full[NST], empty[NST], qfull, sfull[2], pready[2], odone[2], vraw[4], scrubbed[4], drain;
-  __shared__ uint32_t tmem_base, bad_keys[8];
+  float2* ml_s = reinterpret_cast<float2*>(ring + NST * Lo::kItem);
+  __shared__ alignas(16) uint4 clc_s;
+  __shared__ uint64_t full[NST], empty[NST], qfull, qfree, sfull[2], pready[2], odone[2], vraw[8], scrubbed[8], drain,
+      jfull[2], jfree[2], clc, xfull, xfree;
+  __shared__ uint32_t tmem_base, bad_keys[2][8];
   __shared__ int err;
-  __shared__ TileJob job_s;
+  __shared__ TileJob job_s[2];
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int unit = blockIdx.x % a.units;
-  const int kh = unit * a.gp / (a.q_heads / a.heads);
-  const int ctok = SPLIT ? a.tq : 2 * a.tq;  // tokens per CTA
-  int split = 0;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int ctok = SPLIT ? a.tq : 2 * a.tq;  // tokens per job
 
-  // ---- which rows and keys
-  if (PAGED) {
-    const int rest = blockIdx.x / a.units;
-    split = rest / a.row_tiles;
-    if (tid == 0) {
-      const int q0 = (rest % a.row_tiles) * ctok;
-      job_s = TileJob{q0, min(ctok, a.batch - q0), 0, a.key_len, a.key_len - 1};
-    }
-  } else if (warp == 0) {
-    // tiles of the sequences before this one, 32 sequences at a time; a sequence's last tile (the
-    // longest rows) comes first
-    int want = blockIdx.x / a.units;
-    TileJob j{0, 0, 0, 0, -1};
-    for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-      const int s = s0 + lane;
-      int q0 = 0, nq = 0, tiles = 0;
-      if (s < a.n_seqs) {
-        q0 = min(max(a.starts[s], 0), a.q_tokens);
-        nq = max(min(a.starts[s + 1], a.q_tokens) - q0, 0);
-        tiles = (nq + ctok - 1) / ctok;
-      }
-      int upto = tiles;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += x;
-      }
-      const bool mine = want >= upto - tiles && want < upto;
-      const uint32_t who = __ballot_sync(0xffffffffu, mine);
-      if (who) {
-        if (mine) {
-          const int k0 = min(max(a.k_starts[s], 0), a.k_tokens);
-          const int nk = max(min(a.k_starts[s + 1], a.k_tokens) - k0, 0);
-          const int t = (tiles - 1 - (want - (upto - tiles))) * ctok;
-          job_s = TileJob{q0 + t, min(ctok, nq - t), k0, nk, nk - nq + t};
-        }
-        break;
-      }
-      want -= __shfl_sync(0xffffffffu, upto, 31);
-      if (s0 + 32 >= a.n_seqs && lane == 0) job_s = j;
-    }
-  }
   if (tid == 0) {
     for (int i = 0; i < NST; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     mbar_init(&qfull, 1);
+    mbar_init(&qfree, 1);
     mbar_init(&drain, 1);
+    mbar_init(&clc, 1);
+    mbar_init(&xfull, 8);
+    mbar_init(&xfree, 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sfull[i], 1);
       mbar_init(&pready[i], 4);
       mbar_init(&odone[i], 1);
+      mbar_init(&jfull[i], 1);
+      mbar_init(&jfree[i], 11);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       mbar_init(&vraw[i], 1);
       mbar_init(&scrubbed[i], 2);
     }
     fence_mbar_init();
     err = 0;
   }
-  if (tid < 8) bad_keys[tid] = 0u;
-  __syncthreads();
-  const TileJob job = job_s;
-  if (job.tokens == 0) return;  // the grid is sized by a bound: no rows here
+  if (smem_u32(sm) & 1023) {  // the same for all CTAs: fails loudly instead of computing nonsense
+    if (tid == 0) atomicOr(&g_tiles_wait_error, 1u);
+    return;
+  }
   if (warp == 9) tmem_alloc(&tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0);  // S (and P): columns 0, 128; O: columns 256, 384
 
-  // ---- key tiles of each stream: tile0 + u (SPLIT: tile0 + 2u + s), u < steps[s]
-  int tile0 = 0, steps[2], lim_last;
-  {
-    lim_last = PAGED ? job.klen - 1 : job.lim0 + job.tokens - 1;
-    int n = lim_last < 0 ? 0 : lim_last / kTile + 1;
+  auto span_of = [&](const TileJob& job) {
+    TileSpan p;
+    p.tile0 = 0;
+    p.lim_first = PAGED ? job.klen - 1 : job.lim0;
+    p.lim_last = PAGED ? job.klen - 1 : job.lim0 + job.tokens - 1;
+    int n = p.lim_last < 0 ? 0 : p.lim_last / kTile + 1;
     if (PAGED) {
-      tile0 = split * a.tiles_per_split;
-      n = max(min(n, tile0 + a.tiles_per_split) - tile0, 0);
+      p.tile0 = job.split * a.tiles_per_split;
+      n = max(min(n, p.tile0 + a.tiles_per_split) - p.tile0, 0);
     }
     if (SPLIT) {
-      steps[0] = (n + 1) / 2;
-      steps[1] = n / 2;
+      p.steps[0] = (n + 1) / 2;
+      p.steps[1] = n / 2;
     } else {
-      const int lim_a = PAGED ? lim_last : job.lim0 + min(job.tokens, a.tq) - 1;  // stream 0's last row
-      steps[0] = PAGED ? n : (lim_a < 0 ? 0 : lim_a / kTile + 1);
-      steps[1] = job.tokens > a.tq ? n : 0;
+      const int lim_a = job.lim0 + min(job.tokens, a.tq) - 1;  // stream 0's last row
+      p.steps[0] = PAGED ? n : (lim_a < 0 ? 0 : lim_a / kTile + 1);
+      p.steps[1] = job.tokens > a.tq ? n : 0;
     }
-  }
-  steps[0] = __shfl_sync(0xffffffffu, steps[0], 0);  // the same in all threads: keep loops on them uniform
-  steps[1] = __shfl_sync(0xffffffffu, steps[1], 0);
-  const int all = max(steps[0], steps[1]);
-  const int lim_first = PAGED ? job.klen - 1 : job.lim0;
-  auto tile_of = [&](int u, int s) { return SPLIT ? tile0 + 2 * u + s : tile0 + u; };
-  // a tile with a key that some row of the CTA may not see
-  auto hidden_keys = [&](int tile) { return tile * kTile + kTile - 1 > lim_first; };
+    p.all = max(p.steps[0], p.steps[1]);
+    return p;
+  };
+  auto tile_of = [&](const TileSpan& p, int u, int s) { return SPLIT ? p.tile0 + 2 * u + s : p.tile0 + u; };
+  // a tile with a key that some row of the job may not see
+  auto hidden_keys = [&](const TileSpan& p, int tile) { return tile * kTile + kTile - 1 > p.lim_first; };
 
   // The ring holds the tiles in the order in which the MMA warp takes them.  Each role below walks
   // it with the same loop: visit(kind, u, s, first, last) with kind 0 = K, 1 = V; first / last say
   // whether this use takes the item from the ring, and whether it is the last use of it.
-  auto walk = [&](auto&& visit) {
-    if (all == 0) return;
+  auto walk = [&](const TileSpan& p, auto&& visit) {
+    if (p.all == 0) return;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
-      if (steps[s] > 0 && !visit(0, 0, s, SPLIT || s == 0 || steps[0] == 0, SPLIT || s == 1 || steps[1] == 0)) return;
-    for (int u = 0; u < all; ++u)
+      if (p.steps[s] > 0 &&
+          !visit(0, 0, s, SPLIT || s == 0 || p.steps[0] == 0, SPLIT || s == 1 || p.steps[1] == 0))
+        return;
+    for (int u = 0; u < p.all; ++u)
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int kind = 1; kind >= 0; --kind) {
           const int w = kind ? u : u + 1;
-          if (w >= steps[s]) continue;
-          if (!visit(kind, w, s, SPLIT || s == 0 || w >= steps[0], SPLIT || s == 1 || w >= steps[1])) return;
+          if (w >= p.steps[s]) continue;
+          if (!visit(kind, w, s, SPLIT || s == 0 || w >= p.steps[0], SPLIT || s == 1 || w >= p.steps[1])) return;
         }
+  };
+  // The jobs, as the loading warp announces them; work(job, slot) -> go on?
+  auto jobs = [&](auto&& work) {
+    for (int i = 0;; ++i) {
+      const int slot = i & 1;
+      if (!warp_wait(&jfull[slot], (i >> 1) & 1)) return false;
+      TileJob job = job_s[slot];
+      job.tokens = __shfl_sync(0xffffffffu, job.tokens, 0);  // the same in all lanes: keep loops uniform
+      job.klen = __shfl_sync(0xffffffffu, job.klen, 0);
+      job.lim0 = __shfl_sync(0xffffffffu, job.lim0, 0);
+      job.split = __shfl_sync(0xffffffffu, job.split, 0);
+      if (job.tokens < 0) return true;
+      if (!work(job, slot)) return false;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&jfree[slot]);
+    }
   };
 
   // registers: 168 x 384 at launch, shared out again as 56 x 128 + 224 x 256 (the same sum)
   if (warp >= 8) {
    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
    if (warp == 8) {
-    // -------------------------------------------------------------- loads
-    if (all > 0) {
-      if (lane == 0) {
-        const uint32_t bytes = (uint32_t)(a.gp * a.tq * 128 * Lo::kBlocks);
-        const int n_q = SPLIT || job.tokens <= a.tq ? 1 : 2;
-        mbar_arrive_expect_tx(&qfull, n_q * bytes);
-        for (int i = 0; i < n_q; ++i)
-          for (int blk = 0; blk < Lo::kBlocks; ++blk)
-            tma_3d(sm + i * Lo::kItem + blk * Lo::kBlock, &qmap, blk * 64, unit * a.gp, job.q0 + i * a.tq, &qfull);
-      }
-      int it = 0, raw = 0;
-      bool ok = true;
-      walk([&](int kind, int u, int s, bool first, bool) {
-        if (!first) return true;
-        const int slot = it % NST, round = it / NST;
-        ++it;
-        if (round > 0 && !warp_wait(&empty[slot], (round - 1) & 1)) { ok = false; --it; return false; }
-        uint8_t* dst = ring + slot * Lo::kItem;
-        const CUtensorMap* map = kind ? &vmap : &kmap;
-        const int tile = tile_of(u, s);
-        // values to be scrubbed land on a barrier of their own, and their slot counts as filled
-        const bool hidden = kind == 1 && hidden_keys(tile);
-        uint64_t* bar = hidden ? &vraw[raw++ & 3] : &full[slot];
-        if (hidden && lane == 0) mbar_arrive(&full[slot]);
+    // -------------------------------------------------------------- jobs and loads
+    int slot = 0, raw = 0, n_jobs = 0, n_q = 0;  // next ring slot, hidden V tiles, jobs and Q loads so far
+    uint32_t round = 0;                          // times around the ring
+    bool ok = true;
+    int index = blockIdx.x;
+    for (int asked = 0; ok; ++asked) {
+      TileJob job{0, -1, 0, 0, -1, 0, 0};
+      if (index >= 0) {
+        job.unit = index % a.units;
+        const int rest = index / a.units;
+        job.tokens = 0;
         if (PAGED) {
-          // one lane per page of the tile; pages past the last token are not read
-          const int per = kTile >> a.page_shift, left = a.key_len - tile * kTile;
-          const int n = min(per, (left + (1 << a.page_shift) - 1) >> a.page_shift);
-          if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(n * Lo::kBlocks) * (128u << a.page_shift));
-          __syncwarp();
-          if (lane < n) {
-            const int page = min(max(a.table[tile * per + lane], 0), a.n_pages - 1);
-            for (int blk = 0; blk < Lo::kBlocks; ++blk)
-              tma_4d(dst + blk * Lo::kBlock + ((lane * 128) << a.page_shift), map, blk * 64, 0, kh, page, bar);
+          job.split = rest / a.row_tiles;
+          job.q0 = (rest % a.row_tiles) * ctok;
+          job.tokens = min(ctok, a.batch - job.q0);
+          job.klen = a.key_len;
+          job.lim0 = a.key_len - 1;
+        } else {
+          // tiles of the sequences before this one, 32 sequences at a time; a sequence's last tile
+          // (the longest rows) comes first
+          int want = rest;
+          for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+            const int s = s0 + lane;
+            int q0 = 0, nq = 0, tiles = 0;
+            if (s < a.n_seqs) {
+              q0 = min(max(a.starts[s], 0), a.q_tokens);
+              nq = max(min(a.starts[s + 1], a.q_tokens) - q0, 0);
+              tiles = (nq + ctok - 1) / ctok;
+            }
+            int upto = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const int x = __shfl_up_sync(0xffffffffu, upto, o);
+              if (lane >= o) upto += x;
+            }
+            const uint32_t who = __ballot_sync(0xffffffffu, want >= upto - tiles && want < upto);
+            if (who) {
+              const int src = __ffs(who) - 1;
+              const int ss = s0 + src;
+              const int k0 = min(max(a.k_starts[ss], 0), a.k_tokens);
+              const int nk = max(min(a.k_starts[ss + 1], a.k_tokens) - k0, 0);
+              q0 = __shfl_sync(0xffffffffu, q0, src);
+              nq = __shfl_sync(0xffffffffu, nq, src);
+              tiles = __shfl_sync(0xffffffffu, tiles, src);
+              upto = __shfl_sync(0xffffffffu, upto, src);
+              const int t = (tiles - 1 - (want - (upto - tiles))) * ctok;
+              job.q0 = q0 + t;
+              job.tokens = min(ctok, nq - t);
+              job.k0 = k0;
+              job.klen = nk;
+              job.lim0 = nk - nq + t;
+              break;
+            }
+            want -= __shfl_sync(0xffffffffu, upto, 31);
           }
-        } else if (lane == 0) {
-          mbar_arrive_expect_tx(bar, (uint32_t)Lo::kItem);
-          for (int blk = 0; blk < Lo::kBlocks; ++blk)
-            tma_3d(dst + blk * Lo::kBlock, map, blk * 64, kh, job.k0 + tile * kTile, bar);
         }
-        return true;
-      });
-      if (!ok) {
-        err = 1;
-        // copies in flight land before the shared memory is given up
-        mbar_wait(&qfull, 0, kTileWait);
-        for (int i = 0; i < raw; ++i) mbar_wait(&vraw[i & 3], 0, kTileWait);
-        for (int i = max(it - NST, 0); i < it; ++i) mbar_wait(&full[i % NST], (i / NST) & 1, kTileWait);
+      }
+      if (job.tokens != 0) {  // the grid is sized by a bound: 0 tokens are no job
+        const int js = n_jobs & 1;
+        if (n_jobs >= 2 && !(ok = warp_wait(&jfree[js], ((n_jobs >> 1) - 1) & 1))) break;
+        if (lane < 8) bad_keys[js][lane] = 0u;
+        if (lane == 0) job_s[js] = job;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&jfull[js]);
+        ++n_jobs;
+      }
+      if (index < 0) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&clc, 16);
+        clc_ask(&clc_s, &clc);
+      }
+      if (job.tokens > 0) {
+        const TileSpan p = span_of(job);
+        const int kh = job.unit * a.gp / (a.q_heads / a.heads);
+        int nth = 0;
+        walk(p, [&](int kind, int u, int s, bool first, bool) {
+          if (!first) return true;
+          if (nth++ == (p.all > 1 ? 2 : 1)) {
+            // Q after the first key tile(s): its shared memory is free once the last job's last S is
+            if (n_q > 0 && !warp_wait(&qfree, (n_q - 1) & 1)) return ok = false;
+            ++n_q;
+            if (lane == 0) {
+              const uint32_t bytes = (uint32_t)(a.gp * a.tq * 128 * Lo::kBlocks);
+              const int n = SPLIT || job.tokens <= a.tq ? 1 : 2;
+              mbar_arrive_expect_tx(&qfull, n * bytes);
+              for (int i = 0; i < n; ++i)
+                for (int blk = 0; blk < Lo::kBlocks; ++blk)
+                  tma_3d(sm + i * Lo::kItem + blk * Lo::kBlock, &qmap, blk * 64, job.unit * a.gp, job.q0 + i * a.tq, &qfull);
+            }
+          }
+          if (round > 0 && !warp_wait(&empty[slot], (round - 1) & 1)) return ok = false;
+          uint8_t* dst = ring + slot * Lo::kItem;
+          const CUtensorMap* map = kind ? &vmap : &kmap;
+          const int tile = tile_of(p, u, s);
+          // values to be scrubbed land on a barrier of their own, and their slot counts as filled
+          const bool hidden = kind == 1 && hidden_keys(p, tile);
+          uint64_t* bar = hidden ? &vraw[raw++ & 7] : &full[slot];
+          if (hidden && lane == 0) mbar_arrive(&full[slot]);
+          if (PAGED) {
+            // one lane per page of the tile; pages past the last token are not read
+            const int per = kTile >> a.page_shift, left = a.key_len - tile * kTile;
+            const int n = min(per, (left + (1 << a.page_shift) - 1) >> a.page_shift);
+            if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(n * Lo::kBlocks) * (128u << a.page_shift));
+            __syncwarp();
+            if (lane < n) {
+              const int page = min(max(a.table[tile * per + lane], 0), a.n_pages - 1);
+              for (int blk = 0; blk < Lo::kBlocks; ++blk)
+                tma_4d(dst + blk * Lo::kBlock + ((lane * 128) << a.page_shift), map, blk * 64, 0, kh, page, bar);
+            }
+          } else if (lane == 0) {
+            mbar_arrive_expect_tx(bar, (uint32_t)Lo::kItem);
+            for (int blk = 0; blk < Lo::kBlocks; ++blk)
+              tma_3d(dst + blk * Lo::kBlock, map, blk * 64, kh, job.k0 + tile * kTile, bar);
+          }
+          if (++slot == NST) { slot = 0; ++round; }
+          return true;
+        });
+      }
+      const bool told = warp_wait(&clc, asked & 1);
+      ok = ok && told;
+      if (ok) {
+        index = clc_answer(&clc_s);
+        __syncwarp();
+        fence_proxy_async_smem();  // the answer is read before the next one is written
+      }
+    }
+    if (!ok) {
+      err = 1;
+      // copies in flight land before the shared memory is given up
+      if (n_q > 0) warp_wait(&qfull, (n_q - 1) & 1);
+      for (int i = max(raw - 8, 0); i < raw; ++i) warp_wait(&vraw[i & 7], (i >> 3) & 1);
+      for (int i = 0; i < NST; ++i) {
+        const uint32_t uses = round + (i < slot ? 1 : 0);
+        if (uses > 0) warp_wait(&full[i], (uses - 1) & 1);
       }
     }
    } else if (warp == 9) {
@@ -369,26 +488,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // The whole warp runs this loop, converged, with one elected lane around the instructions: their
     // descriptors then stay in uniform registers.  Issued by one lane of a divergent warp the same
     // 4 x 8 products took 3400 cycles a step instead of 2190 (2050 is the tensor cores' own time).
-    if (all > 0) {
-      constexpr uint32_t kIdS = f16_idesc(H::kType, kTile, kTile);
-      constexpr uint32_t kIdO = f16_idesc(H::kType, kTile, D) | (1u << 16);  // B (values) MN-major
-      // descriptors without the address: K-major, and MN-major with the column blocks kBlock apart
-      constexpr uint64_t kDescK = (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-      constexpr uint64_t kDescV = ((uint64_t)(Lo::kBlock >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-      const uint32_t q16 = __shfl_sync(0xffffffffu, smem_u32(sm) >> 4, 0), ring16 = q16 + Lo::kQ / 16;
-      int slot = 0, raw = 0;
-      uint32_t round = 0;
+    constexpr uint32_t kIdS = f16_idesc(H::kType, kTile, kTile);
+    constexpr uint32_t kIdO = f16_idesc(H::kType, kTile, D) | (1u << 16);  // B (values) MN-major
+    // descriptors without the address: K-major, and MN-major with the column blocks kBlock apart
+    constexpr uint64_t kDescK = (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+    constexpr uint64_t kDescV =
+        ((uint64_t)(Lo::kBlock >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+    const uint32_t q16 = __shfl_sync(0xffffffffu, smem_u32(sm) >> 4, 0), ring16 = q16 + Lo::kQ / 16;
+    int slot = 0, raw = 0;
+    uint32_t round = 0, n_q = 0, n_p[2] = {0, 0};
+    const bool fine = jobs([&](const TileJob& job, int) {
+      const TileSpan p = span_of(job);
+      if (p.all == 0) return true;
       int slot_of[2] = {0, 0};  // where the K / V item in use lies
-      bool ok = warp_wait(&qfull, 0);
+      int left = p.steps[0] + p.steps[1];
+      bool ok = warp_wait(&qfull, n_q & 1);
+      ++n_q;
       if (ok)
-        walk([&](int kind, int u, int s, bool first, bool last) {
+        walk(p, [&](int kind, int u, int s, bool first, bool last) {
           if (first) {
             slot_of[kind] = slot;
             if (!warp_wait(&full[slot], round)) return ok = false;
             if (++slot == NST) { slot = 0; round ^= 1u; }
-            if (kind == 1 && hidden_keys(tile_of(u, s)) && !warp_wait(&scrubbed[raw++ & 3], 0)) return ok = false;
+            if (kind == 1 && hidden_keys(p, tile_of(p, u, s))) {
+              if (!warp_wait(&scrubbed[raw & 7], (raw >> 3) & 1)) return ok = false;
+              ++raw;
+            }
           }
-          if (kind == 1 && !warp_wait(&pready[s], u & 1)) return ok = false;
+          if (kind == 1) {
+            if (!warp_wait(&pready[s], n_p[s] & 1)) return ok = false;
+            ++n_p[s];
+          } else {
+            --left;
+          }
           tc_fence_after();
           const uint32_t item16 = ring16 + slot_of[kind] * (Lo::kItem / 16);
           if (elect_one()) {
@@ -400,66 +532,72 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 umma_f16(tb + s * 128, kDescK | (qs16 + off), kDescK | (item16 + off), kIdS, k > 0 ? 1u : 0u);
               }
               umma_commit(&sfull[s]);
+              if (left == 0) umma_commit(&qfree);
             } else {
 #pragma unroll
               for (int k = 0; k < kTile / 16; ++k)
-                umma_f16_ts(tb + 256 + s * 128, tb + s * 128 + k * 8, kDescV | (item16 + k * 128), kIdO, u > 0 || k > 0 ? 1u : 0u);
-              if (u == steps[s] - 1) umma_commit(&odone[s]);
+                umma_f16_ts(tb + 256 + s * 128, tb + s * 128 + k * 8, kDescV | (item16 + k * 128), kIdO,
+                            u > 0 || k > 0 ? 1u : 0u);
+              if (u == p.steps[s] - 1) umma_commit(&odone[s]);
             }
             if (last) umma_commit(&empty[slot_of[kind]]);
           }
           __syncwarp();
           return true;
         });
-      if (!ok) {
-        err = 1;
-        // products in flight end before the tensor memory is given up
-        if (elect_one()) umma_commit(&drain);
-        warp_wait(&drain, 0);
-      }
-    }
+      return ok;
+    });
+    // products and arrivals in flight end before the tensor memory and the barriers are given up
+    if (elect_one()) umma_commit(&drain);
+    __syncwarp();
+    if (!warp_wait(&drain, 0) || !fine) err = 1;
    } else {
     // -------------------------------------------------------------- scrub
     // The product of a zero weight and a value that is not finite would be NaN.  So in tiles with
     // keys that not every row sees, values past the sequence's end are set to zero, and so are rows
     // with a value that is not finite; the latter are remembered, and the rows that do see them get
-    // their share at the end.  Tiles that every row sees whole are left alone.  (At most 256 tokens
-    // per CTA: three such tiles, one barrier each.)
-    int it = 0, raw = 0;
-    bool ok = true;
-    walk([&](int kind, int u, int s, bool first, bool) {
-      if (!first) return true;
-      const int slot = it++ % NST, tile = tile_of(u, s);
-      if (kind == 0 || !hidden_keys(tile)) return true;
-      if (!warp_wait(&vraw[raw & 3], 0)) return ok = false;
-      uint8_t* v = ring + slot * Lo::kItem;
-      const int key0 = tile * kTile;
-      for (int r0 = (warp - 10) * 64; r0 < (warp - 10) * 64 + 64; r0 += 4) {
-        const int r = r0 + (lane >> 3), key = key0 + r;
-        uint4* p = reinterpret_cast<uint4*>(v + r * 128) + (lane & 7);
-        uint32_t odd = 0;
+    // their share at the end.  Tiles that every row sees whole are left alone.
+    int slot = 0, raw = 0;
+    const bool fine = jobs([&](const TileJob& job, int js) {
+      const TileSpan p = span_of(job);
+      bool ok = true;
+      walk(p, [&](int kind, int u, int s, bool first, bool) {
+        if (!first) return true;
+        const int at = slot, tile = tile_of(p, u, s);
+        if (++slot == NST) slot = 0;
+        if (kind == 0 || !hidden_keys(p, tile)) return true;
+        if (!warp_wait(&vraw[raw & 7], (raw >> 3) & 1)) return ok = false;
+        uint8_t* v = ring + at * Lo::kItem;
+        const int key0 = tile * kTile;
+#pragma unroll 4
+        for (int r0 = (warp - 10) * 64; r0 < (warp - 10) * 64 + 64; r0 += 4) {
+          const int r = r0 + (lane >> 3), key = key0 + r;
+          uint4* w = reinterpret_cast<uint4*>(v + r * 128) + (lane & 7);
+          uint32_t odd = 0;
 #pragma unroll
-        for (int blk = 0; blk < Lo::kBlocks; ++blk) {
-          const uint4 x = p[blk * (Lo::kBlock / 16)];
-          odd |= ((x.x & H::kExp) + H::kOne) | ((x.y & H::kExp) + H::kOne) | ((x.z & H::kExp) + H::kOne) |
-                 ((x.w & H::kExp) + H::kOne);
-        }
-        const uint32_t who = __ballot_sync(0xffffffffu, (odd & 0x80008000u) != 0) >> (lane & 24);
-        const bool past = key >= job.klen;
-        if (past || ((who & 0xFFu) && key > lim_first)) {
+          for (int blk = 0; blk < Lo::kBlocks; ++blk) {
+            const uint4 x = w[blk * (Lo::kBlock / 16)];
+            odd |= ((x.x & H::kExp) + H::kOne) | ((x.y & H::kExp) + H::kOne) | ((x.z & H::kExp) + H::kOne) |
+                   ((x.w & H::kExp) + H::kOne);
+          }
+          const uint32_t who = __ballot_sync(0xffffffffu, (odd & 0x80008000u) != 0) >> (lane & 24);
+          const bool past = key >= job.klen;
+          if (past || ((who & 0xFFu) && key > p.lim_first)) {
 #pragma unroll
-          for (int blk = 0; blk < Lo::kBlocks; ++blk) p[blk * (Lo::kBlock / 16)] = make_uint4(0u, 0u, 0u, 0u);
-          const int i = key - max(lim_first + 1, 0);
-          if (!past && (lane & 7) == 0 && i < 256) atomicOr(&bad_keys[i >> 5], 1u << (i & 31));
+            for (int blk = 0; blk < Lo::kBlocks; ++blk) w[blk * (Lo::kBlock / 16)] = make_uint4(0u, 0u, 0u, 0u);
+            const int i = key - max(p.lim_first + 1, 0);
+            if (!past && (lane & 7) == 0 && i < 256) atomicOr(&bad_keys[js][i >> 5], 1u << (i & 31));
+          }
         }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&scrubbed[raw & 3]);
-      ++raw;
-      return true;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&scrubbed[raw & 7]);
+        ++raw;
+        return true;
+      });
+      return ok;
     });
-    if (!ok) err = 1;
+    if (!fine) err = 1;
    }
   } else {
     // -------------------------------------------------------------- softmax
@@ -468,15 +606,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tb + s * 128 + lanes, tO = tb + 256 + s * 128 + lanes;
     const int tok = row / a.gp;                             // token of the row within its tile
-    const int jt = (SPLIT ? 0 : s * a.tq) + tok;            // and within the CTA
-    const bool live = tok < a.tq && jt < job.tokens;
-    const int lim = PAGED ? lim_last : min(job.lim0 + jt, lim_last);  // the last key that the row sees
-    const int lim_min = PAGED ? lim_last : job.lim0 + (SPLIT ? 0 : s * a.tq);
-    const int n = steps[s];
+    const int jt = (SPLIT ? 0 : s * a.tq) + tok;            // and within the job
+    uint32_t n_s = 0, n_o = 0, n_x = 0;                     // steps, jobs with products, joins so far
+    const bool fine = jobs([&](const TileJob& job_now, int js) {
+    int lim, lim_min, n, key_first;  // the last key that the row sees, and the tile's first row; steps
+    {
+      const TileSpan p = span_of(job_now);
+      lim = PAGED ? p.lim_last : min(job_now.lim0 + jt, p.lim_last);
+      lim_min = PAGED ? p.lim_last : job_now.lim0 + (SPLIT ? 0 : s * a.tq);
+      n = p.steps[s];
+      key_first = tile_of(p, 0, s) * kTile;
+    }
     float m = -INFINITY, l = 0.0f;
-    bool ok = true;
-    for (int u = 0; u < n; ++u) {
-      if (!warp_wait(&sfull[s], u & 1)) { ok = false; break; }
+    for (int u = 0; u < n; ++u, ++n_s) {
+      if (!warp_wait(&sfull[s], n_s & 1)) return false;
       tc_fence_after();
       uint32_t x[128];
 #pragma unroll
@@ -484,7 +627,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tm_wait_ld();
 #pragma unroll
       for (int i = 0; i < 4; ++i) tm_tie32(x + 32 * i);
-      const int key0 = tile_of(u, s) * kTile;
+      const int key0 = key_first + u * (SPLIT ? 2 * kTile : kTile);
       if (key0 + kTile - 1 > lim_min) {
         const int seen = lim - key0;
 #pragma unroll
@@ -545,115 +688,133 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&pready[s]);
     }
-    if (ok && n > 0) ok = warp_wait(&odone[s], 0);
-    if (SPLIT && ok && steps[s ^ 1] > 0) ok = warp_wait(&odone[s ^ 1], 0);  // the ring is free
-    if (!ok) err = 1;
-    tc_fence_after();
-    __syncwarp();
 
-    // ---- O of the row, 32 columns at a time
-    const int head = unit * a.gp + row % a.gp;
+    // ---- the row's result: O / l, or in SPLIT mode the two streams' results joined, each warp
+    // taking half of the columns (a warp of either stream reaches the same TMEM lanes)
+    float f0 = 1.0f, f1 = 0.0f;
+    const TileJob job = job_s[js];  // again: it is not held over the steps, where registers are short
+    const TileSpan p = span_of(job);
+    const bool live = tok < a.tq && jt < job.tokens;
+    if (SPLIT) {
+      ml_s[s * kTile + row] = make_float2(m, l);
+      if (n > 0 && !warp_wait(&odone[s], n_o & 1)) return false;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&xfull);  // this stream's O, m and l stand
+      if (!warp_wait(&xfull, n_x & 1)) return false;
+      const float2 z0 = ml_s[row], z1 = ml_s[kTile + row];
+      m = fmaxf(z0.x, z1.x);
+      f0 = z0.x == -INFINITY ? 0.0f : (z0.x == m ? 1.0f : ex2t((z0.x - m) * a.c));
+      f1 = z1.x == -INFINITY ? 0.0f : (z1.x == m ? 1.0f : ex2t((z1.x - m) * a.c));
+      // a stream without a maximum has no weights, or only NaN ones, which count
+      l = (z0.y == 0.0f ? 0.0f : z0.y * f0) + (z1.y == 0.0f ? 0.0f : z1.y * f1);
+    } else if (n > 0 && !warp_wait(&odone[s], n_o & 1)) {
+      return false;
+    }
+    if (n > 0) ++n_o;
+    tc_fence_after();
+    const int head = job.unit * a.gp + row % a.gp;
+    const int64_t t = job.q0 + jt;
+    const float inv = PAGED ? 1.0f : (l > 0.0f || l != l ? 1.0f / l : 0.0f);  // a row without keys gives zeros
     const float mc = m == -INFINITY ? 0.0f : m * a.c;
-    bool any_bad = false;
+    uint32_t bad = 0;
     if (!PAGED) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) any_bad |= bad_keys[i] != 0u;
+      for (int i = 0; i < 8; ++i) bad |= bad_keys[js][i];
     }
-    auto o_chunk = [&](int i, float* o) {
-      if (n > 0) {
-        uint32_t r[32];
-        tm_ld32(tO + 32 * i, r);
+    // where the quad's four rows go
+    uint8_t* dst = nullptr;
+    if (live)
+      dst = PAGED ? reinterpret_cast<uint8_t*>(a.ws_acc + ((t * a.q_heads + head) * a.parts + job.split) * D)
+                  : reinterpret_cast<uint8_t*>(static_cast<T*>(a.out) + t * a.o_stride_t + head * a.o_stride_h);
+    uint8_t* rows[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      rows[j] = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), (lane & 28) + j));
+    // SPLIT: the chunks of even number to stream 0's warps, the others to stream 1's
+#pragma unroll 1
+    for (int i = SPLIT ? s : 0; i < D / 32; i += SPLIT ? 2 : 1) {
+      float o[32];
+      uint32_t r[32];
+      if (SPLIT ? p.steps[0] > 0 : n > 0) {
+        tm_ld32((SPLIT ? tb + 256 + lanes : tO) + 32 * i, r);
         tm_wait_ld();
         tm_tie32(r);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(r[j]);
+        for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(r[j]) * f0;
       } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j) o[j] = 0.0f;
       }
-      if (!PAGED && any_bad && live) {
+      if (SPLIT && p.steps[1] > 0) {
+        tm_ld32(tb + 384 + lanes + 32 * i, r);
+        tm_wait_ld();
+        tm_tie32(r);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(r[j]), f1, o[j]);
+      }
+      if (!PAGED && bad && live) {
         // values that were taken out of the product, for the rows that see them
+        const int kh = job.unit * a.gp / (a.q_heads / a.heads);
         for (int b = 0; b < 256; ++b) {
-          if (!(bad_keys[b >> 5] >> (b & 31) & 1u)) continue;
-          const int key = max(lim_first + 1, 0) + b;
-          if (key > lim || (SPLIT && ((key / kTile - tile0) & 1) != s)) continue;
-          const T* q = static_cast<const T*>(a.q) + (int64_t)(job.q0 + jt) * a.q_stride_t + head * a.q_stride_h;
+          if (!(bad_keys[js][b >> 5] >> (b & 31) & 1u)) continue;
+          const int key = max(p.lim_first + 1, 0) + b;
+          if (key > lim) continue;
+          const T* q = static_cast<const T*>(a.q) + t * a.q_stride_t + head * a.q_stride_h;
           const T* k = static_cast<const T*>(a.k) + (int64_t)(job.k0 + key) * a.k_stride_t + kh * a.k_stride_h;
           const T* v = static_cast<const T*>(a.v) + (int64_t)(job.k0 + key) * a.v_stride_t + kh * a.v_stride_h;
           float dot = 0.0f;
           for (int e = 0; e < D; ++e) dot = fmaf(H::wide(q[e]), H::wide(k[e]), dot);
-          const float p = ex2t(fmaf(dot, a.c, -mc));
+          const float w = ex2t(fmaf(dot, a.c, -mc));
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = fmaf(p, H::wide(v[32 * i + j]), o[j]);
+          for (int j = 0; j < 32; ++j) o[j] = fmaf(w, H::wide(v[32 * i + j]), o[j]);
         }
       }
-    };
-    float* mg = reinterpret_cast<float*>(ring);  // [D / 4][128 rows] float4, then m, l
-    float f_own = 1.0f, f_other = 0.0f;
-    if (SPLIT) {
-      float* ml = mg + kTile * D;
-      if (s == 1) {
+      __syncwarp();
+      if (PAGED) {
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          float o[32];
-          o_chunk(i, o);
+        for (int g = 0; g < 2; ++g) {
+          uint32_t w[16];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            reinterpret_cast<float4*>(mg)[(8 * i + j) * kTile + row] =
-                make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[16 * g + j]);
+          quad_transpose(w, lane);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (rows[j])
+              *reinterpret_cast<uint4*>(rows[j] + 128 * i + 64 * g + 16 * (lane & 3)) =
+                  make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
         }
-        ml[2 * row] = m;
-        ml[2 * row + 1] = l;
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (s == 0) {
-        const float mo = ml[2 * row], lo = ml[2 * row + 1], mm = fmaxf(m, mo);
-        f_own = m == -INFINITY ? 0.0f : (m == mm ? 1.0f : ex2t((m - mm) * a.c));
-        f_other = mo == -INFINITY ? 0.0f : (mo == mm ? 1.0f : ex2t((mo - mm) * a.c));
-        l = l * f_own + lo * f_other;
-        m = mm;
+      } else {
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = H::pack(o[2 * j] * inv, o[2 * j + 1] * inv);
+        quad_transpose(w, lane);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (rows[j])
+            *reinterpret_cast<uint4*>(rows[j] + 64 * i + 16 * (lane & 3)) =
+                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
       }
     }
-    if (!SPLIT || s == 0) {
-      const int64_t t = job.q0 + jt;
-      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;  // a row without keys gives zeros
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        float o[32];
-        o_chunk(i, o);
-        if (SPLIT) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 y = reinterpret_cast<const float4*>(mg)[(8 * i + j) * kTile + row];
-            o[4 * j] = o[4 * j] * f_own + y.x * f_other;
-            o[4 * j + 1] = o[4 * j + 1] * f_own + y.y * f_other;
-            o[4 * j + 2] = o[4 * j + 2] * f_own + y.z * f_other;
-            o[4 * j + 3] = o[4 * j + 3] * f_own + y.w * f_other;
-          }
-        }
-        if (!live) continue;
-        if (PAGED) {
-          float4* dst = reinterpret_cast<float4*>(a.ws_acc + ((t * a.q_heads + head) * a.parts + split) * D + 32 * i);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) dst[j] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + t * a.o_stride_t + head * a.o_stride_h + 32 * i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = H::pack(o[8 * j + 2 * e] * inv, o[8 * j + 2 * e + 1] * inv);
-            dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-      }
-      if (live && PAGED) {
-        a.ws_m[(t * a.q_heads + head) * a.parts + split] = m == -INFINITY ? m : m * a.c;
-        a.ws_l[(t * a.q_heads + head) * a.parts + split] = l;
-      } else if (live && a.lse) {
+    if (live && (!SPLIT || s == 0)) {
+      if (PAGED) {
+        a.ws_m[(t * a.q_heads + head) * a.parts + job.split] = m == -INFINITY ? m : m * a.c;
+        a.ws_l[(t * a.q_heads + head) * a.parts + job.split] = l;
+      } else if (a.lse) {
         a.lse[t * a.q_heads + head] = l > 0.0f || l != l ? m * a.scale + logf(l) : -INFINITY;
       }
     }
+    if (SPLIT) {
+      // both streams have read O, m and l: the next job may write them
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&xfree);
+      if (!warp_wait(&xfree, n_x & 1)) return false;
+      ++n_x;
+    }
+    tc_fence_before();
+    return true;
+    });
+    if (!fine) err = 1;
   }
   __syncwarp();
   if (err && lane == 0) atomicOr(&g_tiles_wait_error, 1u);
