@@ -1,4 +1,6 @@
 // Causal attention of packed prompts: nq_tiles.cuh on row tiles of (token, head) pairs.
+#include <algorithm>
+
 #include "nq_tiles.cuh"
 
 namespace nq {
@@ -37,13 +39,18 @@ cudaError_t prompt_d(const PromptArgs& p, cudaStream_t s) {
   // at most this many tiles of a CTA's tokens: one partly filled tile per sequence
   auto ctas = [&](int tok) { return ((int64_t)p.q_tokens / tok + p.n_seqs) * a.units; };
   // Two row tiles per job share their key tiles.  With one row tile per job, its keys split between
-  // the streams, a job takes half as long: better where that fills the last round of jobs.
+  // the streams, a job has half the steps: better where that fills the last round of jobs, and while
+  // the fixed part of a job (about kFixed steps) does not count twice.  Expected tiles, from the
+  // totals alone: a sequence's last row tile is half empty, its rows see its keys but half of its own.
+  constexpr double kFixed = 1.5;
   const int sms = device_sms();
-  auto rounds = [&](int tok) {  // expected: a sequence's last tile is half empty on average
+  const double steps = (std::max(p.k_tokens, p.q_tokens) - 0.5 * p.q_tokens) / p.n_seqs / kTile + 0.5;
+  auto rounds = [&](int tok) {
     const int64_t jobs = ((int64_t)p.q_tokens / tok + (p.n_seqs + 1) / 2) * a.units;
     return (double)((jobs + sms - 1) / sms);
   };
-  if (2.0 * rounds(2 * a.tq) <= rounds(a.tq)) return run_tiles<T, D, false, false>(qm, km, vm, a, ctas(2 * a.tq), s);
+  const bool split = rounds(a.tq) * (kFixed + 0.5 * steps) < rounds(2 * a.tq) * (kFixed + steps);
+  if (!split) return run_tiles<T, D, false, false>(qm, km, vm, a, ctas(2 * a.tq), s);
   return run_tiles<T, D, false, true>(qm, km, vm, a, ctas(a.tq), s);
 }
 

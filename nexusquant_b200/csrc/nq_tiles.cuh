@@ -730,27 +730,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       rows[j] = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), (lane & 28) + j));
-    // SPLIT: the chunks of even number to stream 0's warps, the others to stream 1's
-#pragma unroll 1
-    for (int i = SPLIT ? s : 0; i < D / 32; i += SPLIT ? 2 : 1) {
+    // All columns of the warp's share in registers at once, 32 at a time in one piece: D of them, or,
+    // with SPLIT, pieces s, s + 2, .. of both streams' O (the odd ones are stream 1's to write).
+    constexpr int kPieces = SPLIT ? (D / 32 + 1) / 2 : D / 32;
+    uint32_t x0[kPieces][32], x1[SPLIT ? kPieces : 1][32];
+    const bool have0 = SPLIT ? p.steps[0] > 0 : n > 0, have1 = SPLIT && p.steps[1] > 0;
+    const uint32_t to0 = (SPLIT ? tb + 256 + lanes + 32 * s : tO);
+    constexpr int kStep = SPLIT ? 64 : 32;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      // (at D = 96 stream 1 has one piece: its second load reads columns that nobody uses)
+      tm_ld32(to0 + kStep * i, x0[i]);
+      if (SPLIT) tm_ld32(to0 + 128 + kStep * i, x1[i]);
+    }
+    tm_wait_ld();
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      tm_tie32(x0[i]);
+      if (SPLIT) tm_tie32(x1[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int col = SPLIT ? 64 * i + 32 * s : 32 * i;
+      if (SPLIT && col >= D) continue;
       float o[32];
-      uint32_t r[32];
-      if (SPLIT ? p.steps[0] > 0 : n > 0) {
-        tm_ld32((SPLIT ? tb + 256 + lanes : tO) + 32 * i, r);
-        tm_wait_ld();
-        tm_tie32(r);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(r[j]) * f0;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = 0.0f;
-      }
-      if (SPLIT && p.steps[1] > 0) {
-        tm_ld32(tb + 384 + lanes + 32 * i, r);
-        tm_wait_ld();
-        tm_tie32(r);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(r[j]), f1, o[j]);
+      for (int j = 0; j < 32; ++j) {
+        o[j] = have0 ? __uint_as_float(x0[i][j]) * f0 : 0.0f;
+        if (SPLIT) o[j] = have1 ? fmaf(__uint_as_float(x1[i][j]), f1, o[j]) : o[j];
       }
       if (!PAGED && bad && live) {
         // values that were taken out of the product, for the rows that see them
@@ -766,7 +773,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int e = 0; e < D; ++e) dot = fmaf(H::wide(q[e]), H::wide(k[e]), dot);
           const float w = ex2t(fmaf(dot, a.c, -mc));
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = fmaf(w, H::wide(v[32 * i + j]), o[j]);
+          for (int j = 0; j < 32; ++j) o[j] = fmaf(w, H::wide(v[col + j]), o[j]);
         }
       }
       __syncwarp();
@@ -780,7 +787,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (rows[j])
-              *reinterpret_cast<uint4*>(rows[j] + 128 * i + 64 * g + 16 * (lane & 3)) =
+              *reinterpret_cast<uint4*>(rows[j] + 4 * col + 64 * g + 16 * (lane & 3)) =
                   make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
         }
       } else {
@@ -791,7 +798,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (rows[j])
-            *reinterpret_cast<uint4*>(rows[j] + 64 * i + 16 * (lane & 3)) =
+            *reinterpret_cast<uint4*>(rows[j] + 2 * col + 16 * (lane & 3)) =
                 make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
       }
     }
