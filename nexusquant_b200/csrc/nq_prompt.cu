@@ -1,5 +1,6 @@
 // Causal attention of packed prompts: nq_tiles.cuh on row tiles of (token, head) pairs.
 #include <algorithm>
+#include <cmath>
 
 #include "nq_tiles.cuh"
 
@@ -46,8 +47,8 @@ cudaError_t prompt_d(const PromptArgs& p, cudaStream_t s) {
   const int sms = device_sms();
   const double steps = (std::max(p.k_tokens, p.q_tokens) - 0.5 * p.q_tokens) / p.n_seqs / kTile + 0.5;
   auto rounds = [&](int tok) {
-    const int64_t jobs = ((int64_t)p.q_tokens / tok + (p.n_seqs + 1) / 2) * a.units;
-    return (double)((jobs + sms - 1) / sms);
+    const double jobs = ((double)p.q_tokens / tok + 0.5 * p.n_seqs) * a.units;
+    return std::max(1.0, std::ceil(jobs / sms));
   };
   const bool split = rounds(a.tq) * (kFixed + 0.5 * steps) < rounds(2 * a.tq) * (kFixed + steps);
   if (!split) return run_tiles<T, D, false, false>(qm, km, vm, a, ctas(2 * a.tq), s);

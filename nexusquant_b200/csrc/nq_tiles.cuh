@@ -65,6 +65,39 @@ __device__ __forceinline__ float ex2t(float x) {
   return r;
 }
 
+// NaN if any operand is.
+__device__ __forceinline__ float max2n(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3n(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^y of a pair on the multiply-add pipe, for y <= 127: y = n + f with n the nearest integer (Cody
+// and Waite's reduction), 2^f by a polynomial of degree 4 with p(0) = 1 (least maximal relative error
+// on [-1/2, 1/2], 2.9e-6 in fp32, fitted for this use), n added to the exponent.  y is held above
+// -127, where the result is 0 or, for a fraction, below 2^-126.
+__device__ __forceinline__ void ex2_poly(u64 y, float& r0, float& r1) {
+  float y0, y1, t0, t1, p0, p1;
+  upk(y, y0, y1);
+  y = pk(fmaxf(y0, -127.0f), fmaxf(y1, -127.0f));
+  const u64 magic = pk(kMagic, kMagic);
+  const u64 t = add2(y, magic);
+  const u64 f = sub2(y, sub2(t, magic));
+  u64 p = fma2(f, pk(0.00958285574f, 0.00958285574f), pk(0.0559064299f, 0.0559064299f));
+  p = fma2(p, f, pk(0.240240991f, 0.240240991f));
+  p = fma2(p, f, pk(0.693124175f, 0.693124175f));
+  p = fma2(p, f, pk(1.0f, 1.0f));
+  upk(t, t0, t1);
+  upk(p, p0, p1);
+  r0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  r1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
 // Bounded wait of a whole warp with one answer for all its lanes.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, kTileWait));
@@ -233,6 +266,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   using Lo = TileLayout<D, SPLIT>;
   using H = Half16<T>;
   constexpr int NST = Lo::kStages;
+  // Of 8 exponentials, how many the multiply-add pipe computes.  A tile at d = 64 has half the products
+  // per exponential: there 2 of 8 take 16384 tokens of 32 heads from 1428 to 1346 us
+  // (4 of 8: 1380).  At d = 96 and 128 they only cost power: 457 -> 461 us, 1669 -> 1683 us.
+  constexpr int kPoly = D == 64 ? 2 : 0;
   extern __shared__ __align__(1024) uint8_t sm[];  // the 128-byte swizzle counts from multiples of 1024
   uint8_t* ring = sm + Lo::kQ;
   float2* ml_s = reinterpret_cast<float2*>(ring + NST * Lo::kItem);
@@ -636,14 +673,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       float mx[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(x[i]), __uint_as_float(x[4 + i]));
+      for (int i = 0; i < 4; ++i) mx[i] = max2n(__uint_as_float(x[i]), __uint_as_float(x[4 + i]));
 #pragma unroll
       for (int j = 8; j < 128; j += 8)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(x[j + i]), __uint_as_float(x[j + 4 + i]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const float mn = fmaxf(m, top);
-      const bool grow = mn > m && !((mn - m) * a.c <= 8.0f);
+        for (int i = 0; i < 4; ++i) mx[i] = max3n(mx[i], __uint_as_float(x[j + i]), __uint_as_float(x[j + 4 + i]));
+      float mn = max2n(m, max2n(max2n(mx[0], mx[1]), max2n(mx[2], mx[3])));
+      // a logit that is NaN or +inf makes the row NaN, as in the formula: through its maximum
+      if (mn == INFINITY) mn = NAN;
+      const bool grow = !(mn <= m) && !((mn - m) * a.c <= 8.0f);
       if (u == 0) {
         m = mn;
       } else if (__any_sync(0xffffffffu, grow)) {
@@ -672,9 +710,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
           float y0, y1;
-          upk(fma2(pk(__uint_as_float(x[64 * i + 2 * j]), __uint_as_float(x[64 * i + 2 * j + 1])), c2, mc2), y0, y1);
-          y0 = ex2t(y0);
-          y1 = ex2t(y1);
+          const u64 y = fma2(pk(__uint_as_float(x[64 * i + 2 * j]), __uint_as_float(x[64 * i + 2 * j + 1])), c2, mc2);
+          if ((j * kPoly) % 8 < kPoly) {  // kPoly of 8 pairs, evenly spread
+            ex2_poly(y, y0, y1);
+          } else {
+            upk(y, y0, y1);
+            y0 = ex2t(y0);
+            y1 = ex2t(y1);
+          }
           sum[j & 1] = add2(sum[j & 1], pk(y0, y1));
           w[j] = H::pack(y0, y1);
         }
