@@ -345,45 +345,80 @@ __global__ void __launch_bounds__(kDecThreads, kDecResident) decode_rows(const D
   }
 }
 
-// One warp per (sequence, head): the parts' sums, in order.
+// One CTA per (sequence, head): warp w takes parts w, w + 4, .., each lane four dimensions, loads of
+// several parts in flight; the warps' sums are added in order.
+constexpr int kComBatch = 4;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(128) decode_combine(const DecodeArgs a, int parts, const DecodeWs w) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= (int64_t)a.batch * a.q_heads) return;
+  __shared__ float f_s[kMaxParts], red[4];
+  __shared__ float4 v_s[4][D / 4];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float *pm = w.m + row * parts, *pl = w.l + row * parts;
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32)
-    if (pl[i] != 0.0f) top = fmaxf(top, pm[i]);
+  const float4* acc = reinterpret_cast<const float4*>(w.acc) + row * parts * (D / 4);
+  constexpr int kOwn = (kMaxParts + 127) / 128;
+  float mi[kOwn], li[kOwn], top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) {
+    const int i = tid + 128 * k;
+    mi[k] = i < parts ? pm[i] : -INFINITY;
+    li[k] = i < parts ? pl[i] : 0.0f;
+    if (li[k] != 0.0f) top = fmaxf(top, mi[k]);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
   float total = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kOwn; ++k) {
+    // a part without tokens has l = 0 and wrote no sums; one that saw a NaN has l = NaN
+    const float f = li[k] == 0.0f ? 0.0f : (mi[k] == top ? 1.0f : ex2t(mi[k] - top));
+    const int i = tid + 128 * k;
+    if (i < parts) f_s[i] = li[k] == 0.0f ? -1.0f : f;
+    total += li[k] == 0.0f ? 0.0f : li[k] * f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) red[warp] = total;
+  __syncthreads();
+  total = (red[0] + red[1]) + (red[2] + red[3]);
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int i0 = 0; i0 < parts; i0 += 32) {
-    float f = 0.0f, lf = 0.0f;
-    if (i0 + lane < parts) {
-      const float x = pm[i0 + lane], li = pl[i0 + lane];
-      f = li == 0.0f ? 0.0f : (x == top ? 1.0f : ex2t(x - top));
-      lf = li == 0.0f ? 0.0f : li * f;
+  for (int i0 = warp; i0 < parts; i0 += 4 * kComBatch) {
+    float4 x[kComBatch];
+    float f[kComBatch];
+#pragma unroll
+    for (int k = 0; k < kComBatch; ++k) {
+      const int i = i0 + 4 * k;
+      f[k] = i < parts ? f_s[i] : -1.0f;
+      x[k] = f[k] != -1.0f && 4 * lane < D ? acc[i * (D / 4) + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    const uint32_t some = __ballot_sync(0xffffffffu, f != 0.0f || lf != lf);
-    for (int i = 0; i < 32 && i0 + i < parts; ++i) {
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      total += __shfl_sync(0xffffffffu, lf, i);
-      if (!(some >> i & 1u)) continue;  // a part without tokens wrote no sums
-      if (4 * lane < D) {
-        const float4 x = reinterpret_cast<const float4*>(w.acc + (row * parts + i0 + i) * D)[lane];
-        v.x = fmaf(x.x, fi, v.x);
-        v.y = fmaf(x.y, fi, v.y);
-        v.z = fmaf(x.z, fi, v.z);
-        v.w = fmaf(x.w, fi, v.w);
-      }
+#pragma unroll
+    for (int k = 0; k < kComBatch; ++k) {
+      if (f[k] == -1.0f) continue;
+      v.x = fmaf(x[k].x, f[k], v.x);
+      v.y = fmaf(x[k].y, f[k], v.y);
+      v.z = fmaf(x[k].z, f[k], v.z);
+      v.w = fmaf(x[k].w, f[k], v.w);
     }
   }
-  const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-  if (4 * lane < D) {
+  if (4 * lane < D) v_s[warp][lane] = v;
+  __syncthreads();
+  if (tid < D / 4) {
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+      const float4 x = v_s[k][tid];
+      v.x += x.x;
+      v.y += x.y;
+      v.z += x.z;
+      v.w += x.w;
+    }
+    const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
     const int64_t b = row / a.q_heads, head = row % a.q_heads;
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.o_stride_b + head * a.o_stride_h + 4 * lane) =
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + b * a.o_stride_b + head * a.o_stride_h + 4 * tid) =
         make_uint2(Half16<T>::pack(v.x * inv, v.y * inv), Half16<T>::pack(v.z * inv, v.w * inv));
   }
 }
@@ -429,12 +464,12 @@ cudaError_t decode_d(const DecodeArgs& a, const DecodePlan& p, void* ws, cudaStr
     if (e != cudaSuccess) return e;
   }
   const int64_t items = (int64_t)a.batch * a.heads * p.own_rt * p.own_splits + (int64_t)a.heads * p.pre_rt * p.pre_splits;
-  if (items > 0x7fffffff) return cudaErrorInvalidValue;
+  if (items > 0x7fffffff || rows > 0x7fffffff) return cudaErrorInvalidValue;
   if (items > 0) {
     if (p.rows == 8) decode_rows<T, D, 8><<<(unsigned)items, kDecThreads, 0, s>>>(a, p, w);
     else decode_rows<T, D, 16><<<(unsigned)items, kDecThreads, 0, s>>>(a, p, w);
   }
-  if (p.parts == 0 || needs_parts(p)) decode_combine<T, D><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a, p.parts, w);
+  if (p.parts == 0 || needs_parts(p)) decode_combine<T, D><<<(unsigned)rows, 128, 0, s>>>(a, p.parts, w);
   return cudaGetLastError();
 }
 
