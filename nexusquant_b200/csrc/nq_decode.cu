@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecResident) decode_rows(const D
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   const int group = a.q_heads / a.heads;
 
+  asm volatile("griddepcontrol.launch_dependents;");  // the join may be scheduled; it waits for these CTAs
   // ---- which rows, which tokens
   int item = blockIdx.x, n, kh, rt, seq = 0, split, part, t_begin;
   const int32_t* table;
@@ -174,6 +175,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecResident) decode_rows(const D
   if (t_begin >= n && p.parts > 1) {  // no tokens here: the part counts for nothing
     int b, head;
     if (tid < ROWS && row_of(tid, b, head)) w.l[((int64_t)b * a.q_heads + head) * p.parts + part] = 0.0f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
 
@@ -198,8 +200,10 @@ __global__ void __launch_bounds__(kDecThreads, kDecResident) decode_rows(const D
     for (int i = 0; i < VH * 4; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.0f;
   }
 
+  int next = t_begin + warp * kGroup < n ? __ldg(table + ((t_begin + warp * kGroup) >> a.page_shift)) : 0;
   for (int t0 = t_begin + warp * kGroup; t0 < n; t0 += kGroup * kDecWarps) {
-    const int page = min(max(__ldg(table + (t0 >> a.page_shift)), 0), a.n_pages - 1);
+    const int page = min(max(next, 0), a.n_pages - 1);
+    if (t0 + kGroup * kDecWarps < n) next = __ldg(table + ((t0 + kGroup * kDecWarps) >> a.page_shift));
     const int64_t base = ((((int64_t)page * a.heads + kh) << a.page_shift) + (t0 & ((1 << a.page_shift) - 1))) * D;
     const T* kp = static_cast<const T*>(a.k_pages) + base;
     const T* vp = static_cast<const T*>(a.v_pages) + base;
@@ -343,6 +347,9 @@ __global__ void __launch_bounds__(kDecThreads, kDecResident) decode_rows(const D
       if (ll != 0.0f) reinterpret_cast<float4*>(w.acc + at * D)[d4] = v;
     }
   }
+  // This grid may have started before attend_tiles ended (it needs nothing from it): it ends after it,
+  // so that whoever waits for this grid waits for both.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // One CTA per (sequence, head): warp w takes parts w, w + 4, .., each lane four dimensions, loads of
@@ -353,6 +360,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) decode_combine(const DecodeArgs a, int parts, const DecodeWs w) {
   __shared__ float f_s[kMaxParts], red[4];
   __shared__ float4 v_s[4][D / 4];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are written
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float *pm = w.m + row * parts, *pl = w.l + row * parts;
@@ -450,6 +458,22 @@ cudaError_t prefix_tiles(const DecodeArgs& d, const DecodePlan& p, const DecodeW
                               : run_tiles<T, D, true, false>(qm, km, vm, a, ctas, s);
 }
 
+// Launch that may start while the kernel before it on the stream still runs (programmatic dependent
+// launch): the kernel itself waits where it needs the other's results.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kern)(P...), int64_t ctas, int threads, cudaStream_t s, A... args) {
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3((unsigned)ctas);
+  c.blockDim = dim3((unsigned)threads);
+  c.stream = s;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kern, P(args)...);
+}
+
 template <typename T, int D>
 cudaError_t decode_d(const DecodeArgs& a, const DecodePlan& p, void* ws, cudaStream_t s) {
   const int64_t rows = (int64_t)a.batch * a.q_heads;
@@ -465,11 +489,17 @@ cudaError_t decode_d(const DecodeArgs& a, const DecodePlan& p, void* ws, cudaStr
   }
   const int64_t items = (int64_t)a.batch * a.heads * p.own_rt * p.own_splits + (int64_t)a.heads * p.pre_rt * p.pre_splits;
   if (items > 0x7fffffff || rows > 0x7fffffff) return cudaErrorInvalidValue;
+  cudaError_t e = cudaSuccess;
   if (items > 0) {
-    if (p.rows == 8) decode_rows<T, D, 8><<<(unsigned)items, kDecThreads, 0, s>>>(a, p, w);
-    else decode_rows<T, D, 16><<<(unsigned)items, kDecThreads, 0, s>>>(a, p, w);
+    auto kern = p.rows == 8 ? decode_rows<T, D, 8> : decode_rows<T, D, 16>;
+    if (p.tile_splits) e = launch_early(kern, items, kDecThreads, s, a, p, w);
+    else kern<<<(unsigned)items, kDecThreads, 0, s>>>(a, p, w);
   }
-  if (p.parts == 0 || needs_parts(p)) decode_combine<T, D><<<(unsigned)rows, 128, 0, s>>>(a, p.parts, w);
+  if (e == cudaSuccess && (p.parts == 0 || needs_parts(p))) {
+    if (p.parts) e = launch_early(decode_combine<T, D>, rows, 128, s, a, p.parts, w);
+    else decode_combine<T, D><<<(unsigned)rows, 128, 0, s>>>(a, p.parts, w);
+  }
+  if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }
 

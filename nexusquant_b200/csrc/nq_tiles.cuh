@@ -283,6 +283,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int ctok = SPLIT ? a.tq : 2 * a.tq;  // tokens per job
 
+  if (PAGED) asm volatile("griddepcontrol.launch_dependents;");  // decode_rows may run beside this grid
   if (tid == 0) {
     for (int i = 0; i < NST; ++i) {
       mbar_init(&full[i], 1);
