@@ -25,6 +25,7 @@ cudaError_t prompt_d(const PromptArgs& p, cudaStream_t s) {
   a.v_stride_t = p.v_stride_t; a.v_stride_h = p.v_stride_h;
   a.o_stride_t = p.o_stride_t; a.o_stride_h = p.o_stride_h;
   a.out = p.out; a.lse = p.lse;
+  a.wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.o_stride_t % 16 == 0 && p.o_stride_h % 16 == 0;
   CUtensorMap qm, km, vm;
   const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)p.q_heads, (cuuint64_t)p.q_tokens};
   const int64_t qs[2] = {p.q_stride_h, p.q_stride_t};

@@ -51,6 +51,7 @@ struct TileArgs {
   const void *q, *k, *v;
   int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, o_stride_t, o_stride_h;
   void* out;
+  bool wide;  // rows of out start at multiples of 32 bytes
   float* lse;
   // shared prefix in pages
   const int32_t* table;
@@ -239,23 +240,17 @@ __device__ __forceinline__ int clc_answer(const uint4* answer) {
   return ok ? (int)x : -1;
 }
 
-// 4 x 4 units of 16 bytes between the four lanes of a quad: afterwards unit j of lane i is unit i of
-// lane j, so that four lanes store 64 consecutive bytes of one row.
-__device__ __forceinline__ void quad_transpose(uint32_t (&w)[16], int lane) {
-#pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    const bool up = lane & o;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j & o) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t send = up ? w[4 * j + e] : w[4 * (j + o) + e];
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, send, o);
-        if (up) w[4 * j + e] = got;
-        else w[4 * (j + o) + e] = got;
-      }
-    }
+// 32 bytes of a row, a whole sector, from one thread: one store where its address allows it.  (Rows
+// exchanged between lanes for coalesced 16-byte stores took 1300 cycles of shuffles a job; twelve
+// prompts of 8191 tokens 87 us against 84.)
+__device__ __forceinline__ void store32(void* p, const uint32_t* w, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
 }
 
@@ -765,15 +760,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
       for (int i = 0; i < 8; ++i) bad |= bad_keys[js][i];
     }
-    // where the quad's four rows go
-    uint8_t* dst = nullptr;
+    uint8_t* dst = nullptr;  // where the row goes
     if (live)
       dst = PAGED ? reinterpret_cast<uint8_t*>(a.ws_acc + ((t * a.q_heads + head) * a.parts + job.split) * D)
                   : reinterpret_cast<uint8_t*>(static_cast<T*>(a.out) + t * a.o_stride_t + head * a.o_stride_h);
-    uint8_t* rows[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      rows[j] = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), (lane & 28) + j));
     // All columns of the warp's share in registers at once, 32 at a time in one piece: D of them, or,
     // with SPLIT, pieces s, s + 2, .. of both streams' O (the odd ones are stream 1's to write).
     constexpr int kPieces = SPLIT ? (D / 32 + 1) / 2 : D / 32;
@@ -820,30 +810,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int j = 0; j < 32; ++j) o[j] = fmaf(w, H::wide(v[col + j]), o[j]);
         }
       }
-      __syncwarp();
+      if (!dst) continue;
       if (PAGED) {
+        uint32_t w[32];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          uint32_t w[16];
+        for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(o[j]);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(o[16 * g + j]);
-          quad_transpose(w, lane);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (rows[j])
-              *reinterpret_cast<uint4*>(rows[j] + 4 * col + 64 * g + 16 * (lane & 3)) =
-                  make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-        }
+        for (int j = 0; j < 4; ++j) store32(dst + 4 * col + 32 * j, w + 8 * j, true);
       } else {
         uint32_t w[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) w[j] = H::pack(o[2 * j] * inv, o[2 * j + 1] * inv);
-        quad_transpose(w, lane);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (rows[j])
-            *reinterpret_cast<uint4*>(rows[j] + 2 * col + 16 * (lane & 3)) =
-                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        for (int j = 0; j < 2; ++j) store32(dst + 2 * col + 32 * j, w + 8 * j, a.wide);
       }
     }
     if (live && (!SPLIT || s == 0)) {

@@ -709,3 +709,15 @@ def test_entry_points_refuse_without_a_gpu():
     assert lib.nq_compact_pages(pool(), 1, one, 2, one, 32, None, 0, one, 1, None) == 0
     assert lib.nq_copy_pages(pool(row=24), one, one, 1, None) == -6
     assert lib.nq_copy_pages(pool(page=20), one, one, 1, None) == -2
+
+
+@gpu
+def test_prompt_rows_of_out_at_any_16_bytes():
+    """out= whose rows start at odd multiples of 16 bytes."""
+    n = 150
+    q, k, v = rand((n, 4, 64), F16, 0), rand((n, 2, 64), F16, 1), rand((n, 2, 64), F16, 2)
+    buf = torch.full((n, 4, 72), 5.0, dtype=F16, device=DEV)
+    out = buf[:, :, 8:]
+    K.attend_prompt(q, k, v, ints([0, 100, n]), out=out)
+    check_prompt(out, None, q, k, v, [0, 100, n], [0, 100, n])
+    assert (buf[:, :, :8] == 5.0).all()
