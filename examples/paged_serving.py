@@ -1,0 +1,146 @@
+"""Serving with a paged cache: packed prompts, eviction, forks, decoding over a shared prefix.
+
+    python examples/paged_serving.py [--layers 4 --prompt 2000 --samples 8 --steps 16 --evict 0.6]
+
+A small random-weight decoder (attention blocks only) runs the way a server would:
+
+  prefill   two prompts of different lengths, packed into one batch: per layer norm_rope_qk norms and
+            rotates queries and keys and stores keys and values into the pages, attend_prompt attends
+  evict     the keys of layer 0 are scored (score_keykey), select_keep picks what stays, and
+            PagePool.compact moves it to fresh pages in all layers at once
+  fork      the first prompt is sampled several times: full pages are shared, the last one copied
+  decode    one token per sample and step: attend_pages reads the shared pages once for all samples
+
+Random weights and synthetic hidden states: the point is the calls, not the text.
+"""
+from __future__ import annotations
+
+import argparse
+import os
+import sys
+import time
+from typing import List
+
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+from nexusquant_b200 import PagePool  # noqa: E402
+from nexusquant_b200 import kernels as K  # noqa: E402
+from nexusquant_b200.pipeline import n_keep_for  # noqa: E402
+
+ROPE_BASE = 10000.0
+EPS = 1e-6
+
+
+class Decoder:
+    """Attention blocks with a fused query-key-value projection and per-head norms."""
+
+    def __init__(self, layers: int = 4, q_heads: int = 16, heads: int = 4, head_dim: int = 128, seed: int = 0,
+                 dtype: torch.dtype = torch.bfloat16, device: str = "cuda"):
+        self.layers, self.hq, self.h, self.d, self.dtype, self.device = layers, q_heads, heads, head_dim, dtype, device
+        self.width = q_heads * head_dim
+        g = torch.Generator(device=device).manual_seed(seed)
+
+        def weight(*shape):
+            return (torch.randn(shape, generator=g, device=device) * shape[0] ** -0.5).to(dtype)
+
+        self.wqkv = [weight(self.width, (q_heads + 2 * heads) * head_dim) for _ in range(layers)]
+        self.wo = [weight(self.width, self.width) for _ in range(layers)]
+        self.norm_q = [torch.ones(head_dim, dtype=dtype, device=device) for _ in range(layers)]
+        self.norm_k = [torch.ones(head_dim, dtype=dtype, device=device) for _ in range(layers)]
+
+    def _project(self, l: int, x: torch.Tensor):
+        qkv = (x @ self.wqkv[l]).view(x.shape[0], self.hq + 2 * self.h, self.d)
+        return qkv[:, :self.hq], qkv[:, self.hq:self.hq + self.h], qkv[:, self.hq + self.h:]
+
+    def _store(self, l: int, x, positions, pool: PagePool, slots, rows: int):
+        q, k, v = self._project(l, x)
+        q, _ = K.norm_rope_qk(q, k, positions, q_weight=self.norm_q[l], k_weight=self.norm_k[l], eps=EPS, v=v,
+                              k_pages=pool.k[l], v_pages=pool.v[l], slots=slots, rope_base=ROPE_BASE, rope_rows=rows)
+        return q, k, v
+
+    def prefill(self, x: torch.Tensor, lens: List[int], pool: PagePool, seqs: List[int]) -> torch.Tensor:
+        """Hidden states [tokens, width] of packed prompts -> the last block's output, the pages filled."""
+        starts = torch.tensor([0] + lens).cumsum(0).to(device=self.device, dtype=torch.int32)
+        positions = torch.cat([torch.arange(n) for n in lens]).to(device=self.device, dtype=torch.int32)
+        slots = torch.cat([pool.extend(s, n) for s, n in zip(seqs, lens)])
+        rows = max(lens)
+        for l in range(self.layers):
+            q, k, v = self._store(l, x, positions, pool, slots, rows)
+            # the prompt attends to its own keys: dense, rotated like the stored ones
+            _, k = K.norm_rope_qk(q, k, positions, k_weight=self.norm_k[l], eps=EPS, rope_base=ROPE_BASE, rope_rows=rows)
+            y = K.attend_prompt(q, k, v, starts)
+            x = x + y.view(x.shape[0], -1) @ self.wo[l]
+        return x
+
+    def step(self, x: torch.Tensor, positions: torch.Tensor, rows: int, pool: PagePool, seqs: List[int]) -> torch.Tensor:
+        """One token per sequence: hidden states [batch, width] -> the last block's output."""
+        slots = pool.extend_each(seqs, 1)
+        batch = pool.batch(seqs)
+        for l in range(self.layers):
+            q, _, _ = self._store(l, x, positions, pool, slots, rows)
+            x = x + pool.attend(q, l, batch).view(x.shape[0], -1) @ self.wo[l]
+        return x
+
+
+def evict(pool: PagePool, seq: int, rate: float, window: int = 32) -> None:
+    """Key-key importance of layer 0, then the top tokens, the first one and the newest stay."""
+    n = pool.length(seq)
+    pages = torch.tensor(pool.pages(seq), device=pool.k.device)
+    keys = pool.k[0][pages].transpose(0, 1).reshape(1, pool.k.shape[2], -1, pool.k.shape[4])[:, :, :n]
+    kept_idx, kept_count = K.select_keep(K.score_keykey(keys, window), window, n_keep_for(n, window, rate))
+    pool.compact([seq], kept_idx, kept_count)
+
+
+def serve(layers=4, prompt=2000, samples=8, steps=16, evict_rate=0.6, q_heads=16, heads=4, head_dim=128, page_size=16,
+          seed=0, verbose=True):
+    """The whole flow; returns the samples' outputs [steps, samples, width], the pool and the sequences."""
+    model = Decoder(layers, q_heads, heads, head_dim, seed)
+    lens = [prompt, max(1, prompt // 3)]
+    need = sum(-(-n // page_size) for n in lens) * 2 + samples * (steps // page_size + 2) + 8
+    pool = PagePool(layers, need, heads, head_dim, page_size=page_size, dtype=model.dtype)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    seqs = [pool.add() for _ in lens]
+    x = model.prefill(torch.randn(sum(lens), model.width, generator=g, device="cuda").to(model.dtype), lens, pool, seqs)
+    if evict_rate > 0:
+        for s in seqs:
+            evict(pool, s, evict_rate)
+    kids = pool.fork(seqs[0], samples)
+    batch = kids + [seqs[1]]
+    positions = [lens[0]] * samples + [lens[1]]
+    h = torch.cat([x[lens[0] - 1:lens[0]].expand(samples, -1), x[-1:]]).contiguous()
+    outs = []
+    torch.cuda.synchronize()
+    began = time.perf_counter()
+    for _ in range(steps):
+        pos = torch.tensor(positions, dtype=torch.int32, device="cuda")
+        noise = torch.randn(h.shape, generator=g, device="cuda").to(h.dtype)  # stands in for the sampled tokens
+        h = torch.nn.functional.layer_norm(h.float(), h.shape[-1:]).to(h.dtype) + noise
+        h = model.step(h, pos, max(positions) + 1, pool, batch)
+        positions = [p + 1 for p in positions]
+        outs.append(h)
+    torch.cuda.synchronize()
+    if verbose:
+        plan = pool.batch(kids)
+        print(f"prompts {lens}, {pool.length(kids[0])} tokens per sample after eviction and {steps} steps, "
+              f"{plan.prefix_len} of them shared by {samples} samples; "
+              f"{(time.perf_counter() - began) / max(1, steps) * 1e3:.2f} ms a step of {layers} layers; "
+              f"{pool.n_pages - pool.free_pages} of {pool.n_pages} pages in use")
+    K.check_device_errors()
+    return torch.stack(outs) if outs else None, pool, batch
+
+
+def main():
+    p = argparse.ArgumentParser(description=__doc__.splitlines()[0])
+    p.add_argument("--layers", type=int, default=4)
+    p.add_argument("--prompt", type=int, default=2000)
+    p.add_argument("--samples", type=int, default=8)
+    p.add_argument("--steps", type=int, default=16)
+    p.add_argument("--evict", type=float, default=0.6)
+    a = p.parse_args()
+    serve(a.layers, a.prompt, a.samples, a.steps, a.evict)
+
+
+if __name__ == "__main__":
+    main()

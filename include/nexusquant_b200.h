@@ -411,8 +411,8 @@ nq_status_t nq_norm_rope_qk(const nq_norm_rope_params_t *params, nq_stream_t str
  * Causal attention of packed sequences: the queries of sequence i are rows seq_starts[i] ..
  * seq_starts[i+1] of q, its keys rows k_starts[i] .. k_starts[i+1] of k / v.  The last query
  * stands at the last key (query r of nq sees keys 0 .. nk - nq + r), so keys may start before the
- * queries.  A query that sees no key gets a zero row (lse -inf).  Starts are ascending device
- * int32, clamped to the tensors.  Keys a query does not see never reach its output, whatever
+ * queries.  A query that sees no key gets a zero row (lse -inf); rows of no sequence are left as
+ * they are.  Starts are ascending device int32, clamped to the tensors.  Keys a query does not see never reach its output, whatever
  * their bits.  fp16 or bf16; the softmax weights are rounded to that type for the second product,
  * sums are fp32.
  */

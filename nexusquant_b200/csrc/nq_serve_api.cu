@@ -49,7 +49,7 @@ nq_status_t decode_args(const nq_attend_pages_params_t* p, nq::DecodeArgs& a) {
   if (p->dtype != NQ_F16 && p->dtype != NQ_BF16) return NQ_ERR_UNSUPPORTED;
   if (!head_dim_ok(p->head_dim) || p->q_heads % p->heads) return NQ_ERR_UNSUPPORTED;
   const int sh = page_shift(p->page_size);
-  if (sh < 0 || p->heads > 65535 || p->batch > 65535) return NQ_ERR_UNSUPPORTED;
+  if (sh < 0) return NQ_ERR_UNSUPPORTED;
   if (!scale_ok(p->scale)) return NQ_ERR_INVALID_ARG;
   if (p->max_len > (int64_t)p->table_width << sh) return NQ_ERR_INVALID_ARG;
   if ((p->max_len || p->prefix_len) && p->n_pages == 0) return NQ_ERR_INVALID_ARG;
@@ -115,7 +115,7 @@ nq_status_t nq_attend_prompt(const nq_attend_prompt_params_t* p, nq_stream_t str
   if (!p || p->n_seqs < 0 || p->q_tokens < 0 || p->k_tokens < 0 || p->q_heads <= 0 || p->heads <= 0)
     return NQ_ERR_INVALID_ARG;
   if (p->dtype != NQ_F16 && p->dtype != NQ_BF16) return NQ_ERR_UNSUPPORTED;
-  if (!head_dim_ok(p->head_dim) || p->q_heads % p->heads || p->q_heads > 65535) return NQ_ERR_UNSUPPORTED;
+  if (!head_dim_ok(p->head_dim) || p->q_heads % p->heads) return NQ_ERR_UNSUPPORTED;
   if (!scale_ok(p->scale)) return NQ_ERR_INVALID_ARG;
   if (p->n_seqs == 0 || p->q_tokens == 0) return NQ_OK;
   if (!p->q || !p->out || !p->seq_starts || !p->k_starts || (p->k_tokens && (!p->k || !p->v)))

@@ -6,7 +6,9 @@ stream.  They replace the reference's GPU entry points in
 nexusquant/kernels/e8_triton.py (e8_quantize_perhead :478, e8_encode :525,
 e8_decode :574) and the torch math the pipelines run per layer.
 
-Tensors are [batch, heads, tokens, head_dim] with a unit innermost stride.
+Tensors are [batch, heads, tokens, head_dim] with a unit innermost stride; the serving operators
+around the cache (norm_rope_qk, attend_prompt, attend_pages, copy_pages, compact_pages) take
+packed tokens [tokens, heads, head_dim] and pages [n_pages, heads, page_size, head_dim].
 """
 from __future__ import annotations
 
@@ -669,21 +671,22 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i:
 _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _rows16(t: torch.Tensor):
+def _rows16(t: torch.Tensor, broadcast: bool = True):
     """(t, address, strides of the two outer dimensions) with 16-byte aligned rows of contiguous
-    elements; t is a contiguous copy where its rows are not."""
+    elements; t is a contiguous copy where its rows are not, or, unless broadcast is allowed, where a
+    stride is 0."""
     ptr, (s0, s1, s2) = t.data_ptr(), t.stride()
-    per = 15 // t.element_size()
-    if ptr & 15 or s2 != 1 or s0 & per or s1 & per:
+    per = 3 if t.dtype is torch.float32 else 7
+    if ptr & 15 or s2 != 1 or s0 & per or s1 & per or not (broadcast or (s0 and s1)):
         t = t.clone(memory_format=torch.contiguous_format)
         ptr, (s0, s1, _) = t.data_ptr(), t.stride()
     return t, ptr, s0, s1
 
 
-def _int32(t: torch.Tensor, dev) -> torch.Tensor:
-    if t.dtype == torch.int32 and t.is_contiguous() and t.device == dev:
+def _int32(t: torch.Tensor, index: int) -> torch.Tensor:
+    if t.dtype is torch.int32 and t.get_device() == index and t.is_contiguous():
         return t
-    return t.to(device=dev, dtype=torch.int32).contiguous()
+    return t.to(device=torch.device("cuda", index), dtype=torch.int32).contiguous()
 
 
 def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], dtypes):
@@ -730,9 +733,9 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dims: int):
 def _out(out: Optional[torch.Tensor], like: torch.Tensor, shape):
     """(out, address, outer strides): a new tensor of the given shape, or the caller's, checked."""
     if out is None:
-        out = torch.empty(shape, dtype=like.dtype, device=like.device)
+        out = like.new_empty(shape)
         return out, out.data_ptr(), shape[1] * shape[2], shape[2]
-    if out.shape != shape or out.dtype != like.dtype or out.device != like.device:
+    if out.shape != shape or out.dtype != like.dtype or out.get_device() != like.get_device():
         raise ValueError("out must have the queries' shape, dtype and device")
     same, ptr, s0, s1 = _rows16(out)
     if same is not out or any(st == 0 and n > 1 for st, n in zip(out.stride(), shape)):
@@ -780,7 +783,7 @@ def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *,
                 positions.max() (a host synchronisation) to size the table.
     Returns (q_out, k_out); k_out is None with pages.  Computed in fp32, rounded once."""
     (n, hq, d), (nk, h, _) = _check_qkv(q, k, v, _DTYPES)
-    dev, dt = q.device, q.dtype
+    index, dt = q.get_device(), q.dtype
     if nk != n or positions.numel() != n:
         raise ValueError(f"{nk} keys and {positions.numel()} positions for {n} queries")
     ko = kos0 = kos1 = vp = vs0 = vs1 = kp = vpp = n_pages = page = slot_p = 0
@@ -788,11 +791,11 @@ def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *,
         if k_pages is None or v_pages is None or v is None or slots is None:
             raise ValueError("storing into pages needs k_pages, v_pages, v and slots")
         n_pages, hp, page, dp = _check_pages(k_pages, v_pages, 4)
-        if k_pages.dtype != dt or k_pages.device != dev or hp != h or dp != d:
+        if k_pages.dtype != dt or k_pages.get_device() != index or hp != h or dp != d:
             raise ValueError("pages must have the keys' dtype, device, heads and head_dim")
         if slots.numel() != n:
             raise ValueError(f"{slots.numel()} slots for {n} tokens")
-        slots = _int32(slots, dev)
+        slots = _int32(slots, index)
         v, vp, vs0, vs1 = _rows16(v)
         k_out, kp, vpp, slot_p = None, k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr()
     elif slots is not None:
@@ -802,7 +805,7 @@ def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *,
     w32 = False
     for w in (q_weight, k_weight):
         if w is not None:
-            if w.numel() != d or w.device != dev:
+            if w.numel() != d or w.get_device() != index:
                 raise ValueError("norm weights must be [head_dim] on the queries' device")
             w32 = w32 or w.dtype != dt
     if w32:
@@ -816,12 +819,12 @@ def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *,
         wk = k_weight.data_ptr()
     q, qp, qs0, qs1 = _rows16(q)
     k, kptr, ks0, ks1 = _rows16(k)
-    positions = _int32(positions, dev)
+    positions = _int32(positions, index)
     if rope_rows is None:
         rope_rows = int(positions.max().item()) + 1 if n else 1
-    cos, sin = TABLES.get(dev, d, rope_base, int(rope_rows), rope_scaling)
+    cos, sin = TABLES.get(q.device, d, rope_base, int(rope_rows), rope_scaling)
     q_out, qo, qos0, qos1 = _out(q_out, q, (n, hq, d))
-    _launch(dev.index, "nq_norm_rope_qk", _NORM_ROPE(
+    _launch(index, "nq_norm_rope_qk", _NORM_ROPE(
         _DTYPES[dt], n, hq, h, d, qp, kptr, vp, qs0, qs1, ks0, ks1, vs0, vs1, wq, wk,
         int(w32 or dt == torch.float32), eps, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
         qo, ko, qos0, qos1, kos0, kos1, kp, vpp, n_pages, page, slot_p))
@@ -844,12 +847,13 @@ def attend_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts:
     k_starts   : the same for k / v when a sequence's keys start before its queries (a later chunk of
                  a prompt); its last query stands at its last key.  None: the same as seq_starts.
     Returns [n, hq, d] (and, with return_lse, the fp32 log of the softmax sums [n, hq]).  A query that
-    sees no key gets zeros and -inf; keys that a query does not see never reach its row."""
+    sees no key gets zeros and -inf; keys that a query does not see never reach its row; rows of no
+    sequence are not written."""
     (n, hq, d), (m, h, _) = _check_qkv(q, k, v, _ATTEND_DTYPES)
-    dev, dt = q.device, q.dtype
+    index, dt = q.get_device(), q.dtype
     if seq_starts.dim() != 1 or seq_starts.numel() < 1:
         raise ValueError("seq_starts must be [n_seqs + 1]")
-    seq_starts = _int32(seq_starts, dev)
+    seq_starts = _int32(seq_starts, index)
     if k_starts is None:
         if m != n:
             raise ValueError(f"{m} keys for {n} queries: give k_starts")
@@ -857,14 +861,14 @@ def attend_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts:
     else:
         if k_starts.shape != seq_starts.shape:
             raise ValueError("k_starts and seq_starts must have the same shape")
-        k_starts = _int32(k_starts, dev)
+        k_starts = _int32(k_starts, index)
     # the copies to shared memory go by strides: tensors broadcast over heads or tokens are written out
-    q, qp, qs0, qs1 = _rows16(q if all(q.stride()) else q.contiguous())
-    k, kp, ks0, ks1 = _rows16(k if all(k.stride()) else k.contiguous())
-    v, vp, vs0, vs1 = _rows16(v if all(v.stride()) else v.contiguous())
+    q, qp, qs0, qs1 = _rows16(q, False)
+    k, kp, ks0, ks1 = _rows16(k, False)
+    v, vp, vs0, vs1 = _rows16(v, False)
     out, op, os0, os1 = _out(out, q, (n, hq, d))
-    lse = torch.empty((n, hq), dtype=torch.float32, device=dev) if return_lse else None
-    _launch(dev.index, "nq_attend_prompt", _ATTEND_PROMPT(
+    lse = q.new_empty((n, hq), dtype=torch.float32) if return_lse else None
+    _launch(index, "nq_attend_prompt", _ATTEND_PROMPT(
         _DTYPES[dt], seq_starts.numel() - 1, n, m, hq, h, d, qp, kp, vp, qs0, qs1, ks0, ks1, vs0, vs1,
         seq_starts.data_ptr(), k_starts.data_ptr(), _logit_scale(scale), op, os0, os1,
         0 if lse is None else lse.data_ptr()))
@@ -888,12 +892,12 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
         raise ValueError("queries must be [batch, heads, head_dim]")
     n_pages, h, page, dp = _check_pages(k_pages, v_pages, 4)
     b, hq, d = q.shape
-    dev, dt = q.device, q.dtype
-    if q.get_device() < 0:
+    index, dt = q.get_device(), q.dtype
+    if index < 0:
         raise RuntimeError(_CUDA_ONLY)
     if dt not in _ATTEND_DTYPES:
         raise TypeError(f"unsupported dtype {dt}")
-    if dt != k_pages.dtype or q.get_device() != k_pages.get_device() or d != dp:
+    if dt != k_pages.dtype or index != k_pages.get_device() or d != dp:
         raise ValueError("queries and pages must share dtype, device and head_dim")
     if h == 0 or hq == 0 or hq % h:
         raise ValueError(f"{hq} query heads are not a multiple of {h} KV heads")
@@ -908,18 +912,18 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     if prefix_len:
         if prefix_len < 0 or prefix_table is None or prefix_table.numel() * page < prefix_len:
             raise ValueError(f"prefix_table does not hold {prefix_len} tokens")
-        prefix_table = _int32(prefix_table, dev)
+        prefix_table = _int32(prefix_table, index)
         pre = prefix_table.data_ptr()
-    tables, lens = _int32(tables, dev), _int32(lens, dev)
-    q, qp, qs0, qs1 = _rows16(q if all(q.stride()) else q.contiguous())
+    tables, lens = _int32(tables, index), _int32(lens, index)
+    q, qp, qs0, qs1 = _rows16(q, False)
     out, op, os0, os1 = _out(out, q, (b, hq, d))
     p = _ATTEND_PAGES(_DTYPES[dt], b, hq, h, d, n_pages, page, qp, qs0, qs1, k_pages.data_ptr(), v_pages.data_ptr(),
                       tables.data_ptr(), width, lens.data_ptr(), max_len, pre, prefix_len, _logit_scale(scale), op, os0,
                       os1)
     nbytes = N.load().nq_attend_pages_workspace_size(p)
     # scratch from torch's allocator each call: it belongs to the current stream, captured or not
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _launch(dev.index, "nq_attend_pages", p, 0 if ws is None else ws.data_ptr(), nbytes)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch(index, "nq_attend_pages", p, 0 if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
@@ -946,9 +950,9 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
             raise ValueError("a destination page is also a source or is written twice")
         if s and not (0 <= min(s + t) and max(s + t) < n_pages):
             raise ValueError(f"page numbers outside the pool of {n_pages}")
-    dev = k_pages.device
-    src, dst = _int32(src, dev), _int32(dst, dev)
-    _launch(dev.index, "nq_copy_pages", pool, src.data_ptr(), dst.data_ptr(), src.numel())
+    index = k_pages.get_device()
+    src, dst = _int32(src, index), _int32(dst, index)
+    _launch(index, "nq_copy_pages", pool, src.data_ptr(), dst.data_ptr(), src.numel())
 
 
 def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, kept_idx: torch.Tensor,
@@ -973,9 +977,9 @@ def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Te
         max_kept = holds
     if not 0 <= max_kept <= holds:
         raise ValueError(f"max_kept {max_kept} above the {holds} that kept_idx and dst_tables hold")
-    dev = k_pages.device
-    tables, dst_tables, kept_idx = _int32(tables, dev), _int32(dst_tables, dev), _int32(kept_idx, dev)
-    kept_count = None if kept_count is None else _int32(kept_count, dev)
-    _launch(dev.index, "nq_compact_pages", pool, b, tables.data_ptr(), tables.shape[1], kept_idx.data_ptr(),
+    index = k_pages.get_device()
+    tables, dst_tables, kept_idx = _int32(tables, index), _int32(dst_tables, index), _int32(kept_idx, index)
+    kept_count = None if kept_count is None else _int32(kept_count, index)
+    _launch(index, "nq_compact_pages", pool, b, tables.data_ptr(), tables.shape[1], kept_idx.data_ptr(),
             kept_idx.shape[1], 0 if kept_count is None else kept_count.data_ptr(),
             int(max_kept), dst_tables.data_ptr(), dst_tables.shape[1])

@@ -116,12 +116,23 @@ class PagePool:
 
     def extend(self, seq: int, n: int) -> torch.Tensor:
         """Reserve the next ``n`` tokens of a sequence; int32 [n] slots (page * page_size + offset)."""
+        return self.extend_each([seq], n)
+
+    def extend_each(self, seqs: Sequence[int], n: int) -> torch.Tensor:
+        """Reserve the next ``n`` tokens of each of several sequences (a decoding step: n = 1); int32
+        [len(seqs) * n] slots, sequence after sequence, in one upload."""
         if n < 0:
             raise ValueError(f"{n} tokens")
-        s, ps = self._get(seq), self.page_size
-        s.pages += self._take(-(-(s.length + n) // ps) - len(s.pages))
-        slots = [s.pages[t // ps] * ps + t % ps for t in range(s.length, s.length + n)]
-        s.length += n
+        if len(set(seqs)) < len(seqs):
+            raise ValueError("a sequence is given twice")
+        ss, ps = [self._get(s) for s in seqs], self.page_size
+        need = [-(-(s.length + n) // ps) - len(s.pages) for s in ss]
+        fresh = iter(self._take(sum(need)))
+        slots: List[int] = []
+        for s, m in zip(ss, need):
+            s.pages += [next(fresh) for _ in range(m)]
+            slots += [s.pages[t // ps] * ps + t % ps for t in range(s.length, s.length + n)]
+            s.length += n
         return self._ints(slots)
 
     def fork(self, seq: int, copies: int = 1) -> List[int]:
@@ -197,9 +208,13 @@ class PagePool:
         ss, ps = [self._get(s) for s in seqs], self.page_size
         shared = 0
         if len(ss) > 1:
-            most = min(s.length // ps for s in ss)
-            while shared < most and all(s.pages[shared] == ss[0].pages[shared] for s in ss):
-                shared += 1
+            most = min(s.length // ps for s in ss) + 1  # first count known not to be shared
+            while most - shared > 1:
+                m = (shared + most) // 2
+                if all(s.pages[:m] == ss[0].pages[:m] for s in ss):
+                    shared = m
+                else:
+                    most = m
         own = [s.length - shared * ps for s in ss]
         return PageBatch(self._padded([s.pages[shared:] for s in ss]), self._ints(own), max(own, default=0),
                          self._ints(ss[0].pages[:shared]) if shared else None, shared * ps)

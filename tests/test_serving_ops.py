@@ -571,6 +571,7 @@ def test_pool_bookkeeping():
     batch = pool.batch([a, e])
     assert (batch.prefix_len, batch.max_len, batch.lens.tolist()) == (0, 33, [33, 17])
     assert batch.tables.tolist() == [[0, 1, 3], [2, 4, 0]]
+    assert pool.batch([e]).prefix_len == 0  # nothing to share with
     pool.free(e)
     with pytest.raises(ValueError):
         pool.free(e)
@@ -586,6 +587,26 @@ def test_pool_bookkeeping():
     with pytest.raises(ValueError):
         pool.compact([a], torch.zeros(1, 50, dtype=torch.int32), torch.tensor([34]))
     assert pool.free_pages == 3
+
+
+def test_pool_steps_and_shared_pages():
+    pool = PagePool(1, 40, 1, 64, page_size=16, device="cpu")
+    a = pool.add()
+    pool.extend(a, 80)
+    kids = pool.fork(a, 3)
+    slots = pool.extend_each([a] + kids, 1).tolist()
+    assert slots == [80, 96, 112, 128] and pool.free_pages == 40 - 9
+    batch = pool.batch([a] + kids)
+    assert (batch.prefix_len, batch.prefix_table.tolist(), batch.lens.tolist()) == (80, [0, 1, 2, 3, 4], [1, 1, 1, 1])
+    pool.extend(kids[0], 40)
+    other = pool.add()
+    pool.extend(other, 100)
+    assert pool.batch([a, other]).prefix_len == 0 and pool.batch([kids[1], kids[2]]).prefix_len == 80
+    with pytest.raises(ValueError):
+        pool.extend_each([a, a], 1)
+    with pytest.raises(PoolExhausted):
+        pool.extend_each([a, other], 16 * 20)
+    assert pool.length(a) == 81 and pool.length(other) == 100
 
 
 @pytest.mark.parametrize("kw", [dict(page_size=8), dict(page_size=24), dict(head_dim=80), dict(n_pages=0)])
@@ -721,3 +742,100 @@ def test_prompt_rows_of_out_at_any_16_bytes():
     K.attend_prompt(q, k, v, ints([0, 100, n]), out=out)
     check_prompt(out, None, q, k, v, [0, 100, n], [0, 100, n])
     assert (buf[:, :, :8] == 5.0).all()
+
+
+# --------------------------------------------------------------------------- together
+@gpu
+def test_example_serves():
+    """examples/paged_serving.py without eviction against the same blocks over dense caches in fp32."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    layers, prompt, samples, steps = 2, 150, 3, 4
+    out, pool, batch = ex.serve(layers, prompt, samples, steps, 0.0, q_heads=8, heads=2, head_dim=64, verbose=False)
+    assert out.shape == (steps, samples + 1, 8 * 64) and out.isfinite().all()
+
+    # the same flow over dense caches, every product and sum in fp32, stored values rounded to bf16
+    model = ex.Decoder(layers, 8, 2, 64, 0)
+    lens = [prompt, prompt // 3]
+    g = torch.Generator(device=DEV).manual_seed(1)
+
+    def normed(x, pos):
+        z, _ = norm_rope_64(x, torch.ones(64, dtype=BF16, device=DEV), torch.tensor(pos, device=DEV), ex.EPS)
+        return z.to(BF16)
+
+    def block(l, x, pos, cache):
+        q, k, v = model._project(l, x)
+        q, k = normed(q, pos), normed(k, pos)
+        kk, vv = (torch.cat([c, n]) for c, n in zip(cache, (k, v)))
+        nq, nk = q.shape[0], kk.shape[0]
+        o, _, _ = attention_64(q, kk, vv, causal(nq, nk))
+        return x + o.to(BF16).reshape(nq, -1) @ model.wo[l], (kk, vv)
+
+    x = torch.randn(sum(lens), 512, generator=g, device=DEV).to(BF16)
+    empty = torch.zeros(0, 2, 64, dtype=BF16, device=DEV)
+    caches, last = [], []
+    for part in x.split(lens):
+        per = []
+        for l in range(layers):
+            part, c = block(l, part, list(range(part.shape[0])), (empty, empty))
+            per.append(c)
+        caches.append(per)
+        last.append(part[-1:])
+    seqs = [[c for c in caches[0]] for _ in range(samples)] + [caches[1]]
+    h = torch.cat([last[0]] * samples + [last[1]])
+    at = [lens[0]] * samples + [lens[1]]
+    for t in range(steps):
+        noise = torch.randn(h.shape, generator=g, device=DEV).to(BF16)
+        h = torch.nn.functional.layer_norm(h.float(), h.shape[-1:]).to(BF16) + noise
+        rows = []
+        for i in range(samples + 1):
+            r = h[i:i + 1]
+            for l in range(layers):
+                r, seqs[i][l] = block(l, r, [at[i] + t], seqs[i][l])
+            rows.append(r)
+        h = torch.cat(rows)
+        # bf16 activations through 2 (layers) x (t + 1) blocks, each rounding a few values to 2^-8
+        err = (out[t].double() - h.double()).norm() / h.double().norm()
+        assert err < 2 * (t + 1) * 4 * 2.0 ** -8, (t, float(err))
+        h = out[t]  # go on from the same state
+
+
+@gpu
+def test_example_evicts():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_serving.py")
+    spec = importlib.util.spec_from_file_location("paged_serving", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    out, pool, batch = ex.serve(2, 400, 4, 3, 0.6, q_heads=8, heads=2, head_dim=64, verbose=False)
+    assert out.isfinite().all()
+    n = 1 + 32 + ex.n_keep_for(400, 32, 0.6)
+    assert [pool.length(s) for s in batch[:-1]] == [n + 3] * 4
+
+
+@gpu
+@pytest.mark.parametrize("b,prefix", [(3, 100), (40, 700)])
+def test_decode_in_a_cuda_graph(b, prefix):
+    """Captured once, replayed with new queries and lengths (the kernels of a call start early)."""
+    lens = [(7 * i) % 60 for i in range(b)]
+    q, kp, vp, tables, ln, tp, shared, own = decode_case(b, prefix, [64] * b, 8, 2, 128, F16, 16, seed=b)
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=prefix, max_len=64, out=out)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.attend_pages(q, kp, vp, tables, ln, prefix_table=tp, prefix_len=prefix, max_len=64, out=out)
+    for seed in (1, 2):
+        q.copy_(rand(q.shape, F16, seed))
+        lens = [(7 * i + seed) % 65 for i in range(b)]
+        ln.copy_(ints(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_decode(out, q, shared, [(k[:n], v[:n]) for (k, v), n in zip(own, lens)])
