@@ -41,18 +41,21 @@ cudaError_t prompt_d(const PromptArgs& p, cudaStream_t s) {
   // at most this many tiles of a CTA's tokens: one partly filled tile per sequence
   auto ctas = [&](int tok) { return ((int64_t)p.q_tokens / tok + p.n_seqs) * a.units; };
   // Two row tiles per job share their key tiles.  With one row tile per job, its keys split between
-  // the streams, a job has half the steps: better where that fills the last round of jobs, and while
-  // the fixed part of a job (about kFixed steps) does not count twice.  Expected tiles, from the
-  // totals alone: a sequence's last row tile is half empty, its rows see its keys but half of its own.
-  constexpr double kFixed = 1.5;
+  // the streams, a job has half the steps, but the fixed part of a job (about kFixed steps) counts
+  // twice: better while there are few jobs.  Expected time in steps, from the totals alone: at least the
+  // longest job; and the jobs' sum over the SMs, with a last round that is not full.  Measured (us, two
+  // tiles / one): 32 / 8 heads of 128: 512 tokens 16.8 / 14.6, 2048 equal, 4096 118 / 135, 512 after
+  // 8000 cached ones 138 / 74; twelve prompts of 8263 tokens 98 / 121.
+  constexpr double kFixed = 2.0;
   const int sms = device_sms();
-  const double steps = (std::max(p.k_tokens, p.q_tokens) - 0.5 * p.q_tokens) / p.n_seqs / kTile + 0.5;
-  auto rounds = [&](int tok) {
-    const double jobs = ((double)p.q_tokens / tok + 0.5 * p.n_seqs) * a.units;
-    return std::max(1.0, std::ceil(jobs / sms));
+  const double lo = std::max(0.0, (double)p.k_tokens - p.q_tokens) / p.n_seqs / kTile;  // steps of a sequence's first rows
+  const double hi = (double)p.k_tokens / p.n_seqs / kTile;                              // and of its last
+  auto expected = [&](int tok, double part) {  // part: of a row tile's key tiles, how many are steps
+    const double jobs = ((double)p.q_tokens / tok + 0.5 * p.n_seqs) * a.units, rounds = jobs / sms;
+    const double all = rounds * (part * (0.5 * (lo + hi) + 0.5) + kFixed) + (std::ceil(rounds) - rounds) * (part * lo + kFixed);
+    return std::max(part * (hi + 0.5) + kFixed, all);
   };
-  const bool split = rounds(a.tq) * (kFixed + 0.5 * steps) < rounds(2 * a.tq) * (kFixed + steps);
-  if (!split) return run_tiles<T, D, false, false>(qm, km, vm, a, ctas(2 * a.tq), s);
+  if (expected(2 * a.tq, 1.0) <= expected(a.tq, 0.5)) return run_tiles<T, D, false, false>(qm, km, vm, a, ctas(2 * a.tq), s);
   return run_tiles<T, D, false, true>(qm, km, vm, a, ctas(a.tq), s);
 }
 

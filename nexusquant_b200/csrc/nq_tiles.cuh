@@ -447,10 +447,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ++n_jobs;
       }
       if (index < 0) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&clc, 16);
-        clc_ask(&clc_s, &clc);
-      }
       if (job.tokens > 0) {
         const TileSpan p = span_of(job);
         const int kh = job.unit * a.gp / (a.q_heads / a.heads);
@@ -498,8 +494,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           return true;
         });
       }
-      const bool told = warp_wait(&clc, asked & 1);
-      ok = ok && told;
+      if (!ok) break;
+      // The next job is asked for when this one's last tiles are on their way, about two steps before its
+      // end.  (Asked for at its start, the longest first jobs also took the longest second ones: 4096
+      // tokens of 16 / 2 heads of 64, 84 us instead of 63.)
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&clc, 16);
+        clc_ask(&clc_s, &clc);
+      }
+      ok = warp_wait(&clc, asked & 1);
       if (ok) {
         index = clc_answer(&clc_s);
         __syncwarp();
