@@ -51,7 +51,10 @@ cudaError_t prompt_d(const PromptArgs& p, cudaStream_t s) {
   const double lo = std::max(0.0, (double)p.k_tokens - p.q_tokens) / p.n_seqs / kTile;  // steps of a sequence's first rows
   const double hi = (double)p.k_tokens / p.n_seqs / kTile;                              // and of its last
   auto expected = [&](int tok, double part) {  // part: of a row tile's key tiles, how many are steps
-    const double jobs = ((double)p.q_tokens / tok + 0.5 * p.n_seqs) * a.units, rounds = jobs / sms;
+    // a sequence's last row tile is half full, unless all may be of one length that fills them
+    const bool even = p.q_tokens % ((int64_t)p.n_seqs * tok) == 0;
+    const double tiles = (double)p.q_tokens / tok + (even ? 0.0 : 0.5 * p.n_seqs);
+    const double rounds = std::max<double>(tiles, p.n_seqs) * a.units / sms;
     const double all = rounds * (part * (0.5 * (lo + hi) + 0.5) + kFixed) + (std::ceil(rounds) - rounds) * (part * lo + kFixed);
     return std::max(part * (hi + 0.5) + kFixed, all);
   };

@@ -839,3 +839,14 @@ def test_decode_in_a_cuda_graph(b, prefix):
         graph.replay()
         torch.cuda.synchronize()
         check_decode(out, q, shared, [(k[:n], v[:n]) for (k, v), n in zip(own, lens)])
+
+
+@gpu
+@pytest.mark.parametrize("n_seqs", [2, 32, 33, 70])
+def test_prompt_many_sequences(n_seqs):
+    """Sequences of many lengths, some empty: each row once, whatever the order of the work."""
+    lens = [(37 * i * i + 11 * i) % 260 for i in range(n_seqs)]
+    klens = [n + (5 * i) % 40 for i, n in enumerate(lens)]
+    q, k, v, at, atk = prompt_case(lens, klens, 8, 2, 64, BF16, seed=n_seqs)
+    out = K.attend_prompt(q, k, v, ints(at), k_starts=ints(atk))
+    check_prompt(out, None, q, k, v, at, atk)
