@@ -22,7 +22,20 @@
 // A CTA stays and takes further jobs (row tiles x key range x KV head): it cancels the launch of a
 // CTA that has not started and does that one's work (cluster launch control), so the hardware's
 // order of the grid is kept.  The next job's Q, K and V are loaded, and its first S computed, while
-// the softmax warps still write the last one's rows.
+// the softmax warps still write the last one's rows.  (One launch a job: 1777 us instead of 1647 for
+// 16384 tokens of 32 / 8 heads of 128, bf16.)
+//
+// What bounds it.  A step (two row tiles x 128 keys) is 4 x 8 products of 128 x 128 x 16: 2050 cycles
+// of the tensor cores at D = 128; its 32768 exponentials take 2050 cycles of the special-function
+// units (4 a cycle and scheduler).  Measured: about 2900 cycles, since a stream's chain (read S 70,
+// maximum 330, weights 1300, then its two products 1024 and their hand-over 150) leaves each unit idle
+// a quarter of the time.  Long prompts are bound by power instead: 16384 tokens of 32 / 8 heads run
+// at 1330 TFLOP/s for milliseconds and at 1140-1190 for seconds (1.49 GHz, 990 W; the measured peaks
+// of a plain matrix product are 1665 and 1425).  Short sequences are bound by what a job costs beside
+// its steps, about 5000 cycles (the last product, the rows' store, the first tile's chain).
+// Tried and slower: exponentials against the old maximum, 64 keys at a time (97 -> 104 us for twelve
+// prompts of 8191 tokens); two threads a row (101 us, S read twice to fit the registers); separate
+// warps for the store (84 -> 83 us, but 1631 -> 1656 for the long prompt).
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -40,6 +53,7 @@ namespace {
 constexpr int kTile = 128;         // rows of a row tile, keys of a key tile
 constexpr int kTileThreads = 384;
 constexpr uint32_t kTileWait = 1u << 22;  // tries of a bounded wait
+constexpr uint32_t kJobWait = 1u << 25;   // and of one that may last as long as a job (millions of keys)
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct TileArgs {
@@ -100,8 +114,8 @@ __device__ __forceinline__ void ex2_poly(u64 y, float& r0, float& r1) {
 }
 
 // Bounded wait of a whole warp with one answer for all its lanes.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, kTileWait));
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t tries = kTileWait) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, tries));
 }
 
 // One lane of a converged warp.
@@ -363,7 +377,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   auto jobs = [&](auto&& work) {
     for (int i = 0;; ++i) {
       const int slot = i & 1;
-      if (!warp_wait(&jfull[slot], (i >> 1) & 1)) return false;
+      if (!warp_wait(&jfull[slot], (i >> 1) & 1, kJobWait)) return false;
       TileJob job = job_s[slot];
       job.tokens = __shfl_sync(0xffffffffu, job.tokens, 0);  // the same in all lanes: keep loops uniform
       job.klen = __shfl_sync(0xffffffffu, job.klen, 0);
@@ -439,7 +453,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       if (job.tokens != 0) {  // the grid is sized by a bound: 0 tokens are no job
         const int js = n_jobs & 1;
-        if (n_jobs >= 2 && !(ok = warp_wait(&jfree[js], ((n_jobs >> 1) - 1) & 1))) break;
+        if (n_jobs >= 2 && !(ok = warp_wait(&jfree[js], ((n_jobs >> 1) - 1) & 1, kJobWait))) break;
         if (lane < 8) bad_keys[js][lane] = 0u;
         if (lane == 0) job_s[js] = job;
         __syncwarp();
@@ -602,7 +616,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int at = slot, tile = tile_of(p, u, s);
         if (++slot == NST) slot = 0;
         if (kind == 0 || !hidden_keys(p, tile)) return true;
-        if (!warp_wait(&vraw[raw & 7], (raw >> 3) & 1)) return ok = false;
+        if (!warp_wait(&vraw[raw & 7], (raw >> 3) & 1, kJobWait)) return ok = false;
         uint8_t* v = ring + at * Lo::kItem;
         const int key0 = tile * kTile;
 #pragma unroll 4
