@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecResident) decode_rows(const D
   if (t_begin >= n && p.parts > 1) {  // no tokens here: the part counts for nothing
     int b, head;
     if (tid < ROWS && row_of(tid, b, head)) w.l[((int64_t)b * a.q_heads + head) * p.parts + part] = 0.0f;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");  // see the end
     return;
   }
 
@@ -358,9 +358,9 @@ __global__ void __launch_bounds__(kDecThreads, kDecResident) decode_rows(const D
       if (ll != 0.0f) reinterpret_cast<float4*>(w.acc + at * D)[d4] = v;
     }
   }
-  // This grid may have started before attend_tiles ended (it needs nothing from it): it ends after it,
-  // so that whoever waits for this grid waits for both.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // This grid may have started before attend_tiles ended (it needs nothing from it): its first CTA, and so
+  // the grid, ends after it, so that whoever waits for this grid waits for both.
+  if (blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // One CTA per (sequence, head): warp w takes parts w, w + 4, .., each lane four dimensions, loads of
