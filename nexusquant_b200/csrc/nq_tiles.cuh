@@ -205,6 +205,17 @@ struct Half16<__nv_bfloat16> {
   static __device__ __forceinline__ float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
 };
 
+// TMEM columns.  At D = 64 the weights P have columns of their own (kAhead): S is free as soon as the
+// softmax warps have read it, and the next S is computed while they work on this one (16384 tokens of
+// 32 / 8 heads 1311 -> 1235 us).  At D = 96 and 128 there is no room for that.
+template <int D>
+struct TileTmem {
+  static constexpr bool kAhead = D <= 64;
+  static __device__ __forceinline__ uint32_t s(int stream) { return stream * 128; }
+  static __device__ __forceinline__ uint32_t o(int stream) { return 256 + stream * (kAhead ? 64 : 128); }
+  static __device__ __forceinline__ uint32_t p(int stream) { return kAhead ? 384 + stream * 64 : stream * 128; }
+};
+
 template <int D, bool SPLIT>
 struct TileLayout {
   static constexpr int kBlocks = (D + 63) / 64;          // column blocks of 64 elements (128 bytes)
@@ -274,6 +285,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                  const __grid_constant__ CUtensorMap vmap, const TileArgs a) {
   using Lo = TileLayout<D, SPLIT>;
   using H = Half16<T>;
+  using Tm = TileTmem<D>;
+  constexpr bool AHEAD = Tm::kAhead;
   constexpr int NST = Lo::kStages;
   // Of 8 exponentials, how many the multiply-add pipe computes.  A tile at d = 64 has half the products
   // per exponential: there 2 of 8 take 16384 tokens of 32 heads from 1428 to 1346 us
@@ -283,7 +296,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* ring = sm + Lo::kQ;
   float2* ml_s = reinterpret_cast<float2*>(ring + NST * Lo::kItem);
   __shared__ alignas(16) uint4 clc_s;
-  __shared__ uint64_t full[NST], empty[NST], qfull, qfree, sfull[2], pready[2], odone[2], vraw[8], scrubbed[8], drain,
+  __shared__ uint64_t full[NST], empty[NST], qfull, qfree, sfull[2], sread[2], pready[2], pvdone[2], odone[2], vraw[8], scrubbed[8], drain,
       jfull[2], jfree[2], clc, xfull, xfree;
   __shared__ uint32_t tmem_base, bad_keys[2][8];
   __shared__ int err;
@@ -306,7 +319,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     mbar_init(&xfree, 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sfull[i], 1);
+      mbar_init(&sread[i], 4);
       mbar_init(&pready[i], 4);
+      mbar_init(&pvdone[i], 1);
       mbar_init(&odone[i], 1);
       mbar_init(&jfull[i], 1);
       mbar_init(&jfree[i], 11);
@@ -326,7 +341,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0);  // S (and P): columns 0, 128; O: columns 256, 384
+  const uint32_t tb = __shfl_sync(0xffffffffu, tmem_base, 0);
 
   auto span_of = [&](const TileJob& job) {
     TileSpan p;
@@ -359,16 +374,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   auto walk = [&](const TileSpan& p, auto&& visit) {
     if (p.all == 0) return;
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (p.steps[s] > 0 &&
-          !visit(0, 0, s, SPLIT || s == 0 || p.steps[0] == 0, SPLIT || s == 1 || p.steps[1] == 0))
-        return;
+    for (int w = 0; w < (AHEAD ? 2 : 1); ++w)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (p.steps[s] > w &&
+            !visit(0, w, s, SPLIT || s == 0 || p.steps[0] <= w, SPLIT || s == 1 || p.steps[1] <= w))
+          return;
     for (int u = 0; u < p.all; ++u)
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int kind = 1; kind >= 0; --kind) {
-          const int w = kind ? u : u + 1;
+          const int w = kind ? u : u + (AHEAD ? 2 : 1);
           if (w >= p.steps[s]) continue;
           if (!visit(kind, w, s, SPLIT || s == 0 || w >= p.steps[0], SPLIT || s == 1 || w >= p.steps[1])) return;
         }
@@ -546,7 +563,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         ((uint64_t)(Lo::kBlock >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
     const uint32_t q16 = __shfl_sync(0xffffffffu, smem_u32(sm) >> 4, 0), ring16 = q16 + Lo::kQ / 16;
     int slot = 0, raw = 0;
-    uint32_t round = 0, n_q = 0, n_p[2] = {0, 0};
+    uint32_t round = 0, n_q = 0, n_p[2] = {0, 0}, n_r[2] = {0, 0};
     const bool fine = jobs([&](const TileJob& job, int) {
       const TileSpan p = span_of(job);
       if (p.all == 0) return true;
@@ -570,6 +587,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             ++n_p[s];
           } else {
             --left;
+            if (AHEAD) {
+              // S of the step before has been read (also of the last job's last one: counted by job)
+              if (n_r[s] > 0 && !warp_wait(&sread[s], (n_r[s] - 1) & 1)) return ok = false;
+              ++n_r[s];
+            }
           }
           tc_fence_after();
           const uint32_t item16 = ring16 + slot_of[kind] * (Lo::kItem / 16);
@@ -579,15 +601,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
               for (int k = 0; k < D / 16; ++k) {
                 const uint32_t off = (k >> 2) * (Lo::kBlock / 16) + (k & 3) * 2;
-                umma_f16(tb + s * 128, kDescK | (qs16 + off), kDescK | (item16 + off), kIdS, k > 0 ? 1u : 0u);
+                umma_f16(tb + Tm::s(s), kDescK | (qs16 + off), kDescK | (item16 + off), kIdS, k > 0 ? 1u : 0u);
               }
               umma_commit(&sfull[s]);
               if (left == 0) umma_commit(&qfree);
             } else {
 #pragma unroll
               for (int k = 0; k < kTile / 16; ++k)
-                umma_f16_ts(tb + 256 + s * 128, tb + s * 128 + k * 8, kDescV | (item16 + k * 128), kIdO,
+                umma_f16_ts(tb + Tm::o(s), tb + Tm::p(s) + k * 8, kDescV | (item16 + k * 128), kIdO,
                             u > 0 || k > 0 ? 1u : 0u);
+              if (AHEAD) umma_commit(&pvdone[s]);
               if (u == p.steps[s] - 1) umma_commit(&odone[s]);
             }
             if (last) umma_commit(&empty[slot_of[kind]]);
@@ -654,7 +677,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int s = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tb + s * 128 + lanes, tO = tb + 256 + s * 128 + lanes;
+    const uint32_t tS = tb + Tm::s(s) + lanes, tO = tb + Tm::o(s) + lanes, tP = tb + Tm::p(s) + lanes;
     const int tok = row / a.gp;                             // token of the row within its tile
     const int jt = (SPLIT ? 0 : s * a.tq) + tok;            // and within the job
     uint32_t n_s = 0, n_o = 0, n_x = 0;                     // steps, jobs with products, joins so far
@@ -677,6 +700,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       tm_wait_ld();
 #pragma unroll
       for (int i = 0; i < 4; ++i) tm_tie32(x + 32 * i);
+      if (AHEAD) {  // S may be written again
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sread[s]);
+      }
       const int key0 = key_first + u * (SPLIT ? 2 * kTile : kTile);
       if (key0 + kTile - 1 > lim_min) {
         const int seen = lim - key0;
@@ -695,10 +723,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // a logit that is NaN or +inf makes the row NaN, as in the formula: through its maximum
       if (mn == INFINITY) mn = NAN;
       const bool grow = !(mn <= m) && !((mn - m) * a.c <= 8.0f);
+      if (AHEAD && n_s > 0) {  // the product before this step has read P and written O
+        if (!warp_wait(&pvdone[s], (n_s - 1) & 1)) return false;
+        tc_fence_after();
+      }
       if (u == 0) {
         m = mn;
       } else if (__any_sync(0xffffffffu, grow)) {
-        // S of this step is complete, so the product before it is too: O is at rest
+        // the product before this step is complete (without AHEAD: since S of this step is): O is at rest
         const float f = !grow ? 1.0f : (m == -INFINITY ? 0.0f : ex2t((m - mn) * a.c));
         if (grow) m = mn;
         l *= f;
@@ -734,7 +766,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           sum[j & 1] = add2(sum[j & 1], pk(y0, y1));
           w[j] = H::pack(y0, y1);
         }
-        tm_st32(tS + 32 * i, w);
+        tm_st32(tP + 32 * i, w);
       }
       float s0, s1;
       upk(add2(sum[0], sum[1]), s0, s1);
@@ -786,13 +818,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr int kPieces = SPLIT ? (D / 32 + 1) / 2 : D / 32;
     uint32_t x0[kPieces][32], x1[SPLIT ? kPieces : 1][32];
     const bool have0 = SPLIT ? p.steps[0] > 0 : n > 0, have1 = SPLIT && p.steps[1] > 0;
-    const uint32_t to0 = (SPLIT ? tb + 256 + lanes + 32 * s : tO);
+    const uint32_t to0 = (SPLIT ? tb + Tm::o(0) + lanes + 32 * s : tO);
     constexpr int kStep = SPLIT ? 64 : 32;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       // (at D = 96 stream 1 has one piece: its second load reads columns that nobody uses)
       tm_ld32(to0 + kStep * i, x0[i]);
-      if (SPLIT) tm_ld32(to0 + 128 + kStep * i, x1[i]);
+      if (SPLIT) tm_ld32(to0 + (Tm::o(1) - Tm::o(0)) + kStep * i, x1[i]);
     }
     tm_wait_ld();
 #pragma unroll
