@@ -3,16 +3,19 @@
 The shared library is built in-tree (``make -C nexusquant_b200/csrc``, or
 ``__graft_entry__.build()``) into ``nexusquant_b200/_lib/``.  There is no
 fallback: if the library is missing, or the tensors handed to an entry point
-are not CUDA tensors, the call raises.
+are not CUDA tensors, the call raises.  ``front()`` is the compiled front end of
+the serving operators, built beside it.
 """
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libnexusquant_b200.so")
+FRONT_PATH = os.path.join(_HERE, "_lib", "nq_front.so")
 
 c_i32 = ctypes.c_int32
 c_i64 = ctypes.c_int64
@@ -112,7 +115,7 @@ _PROTOS = {
     "nq_unpack_nibbles": (c_i32, [c_vp, c_i64, c_i32, c_vp, c_vp]),
     "nq_merge_apply": (c_i32, [ctypes.POINTER(c_vp), c_i32, c_i32, c_i32, c_i32, c_i32, c_i64, c_i64, c_vp, c_vp,
                                c_i32, c_vp, c_vp, c_vp]),
-    # parameter structs of the serving operators come packed, as bytes (kernels.py)
+    # parameter structs of the serving operators come packed, as bytes; kernels.py calls them through front()
     "nq_norm_rope_qk": (c_i32, [c_vp, c_vp]),
     "nq_attend_prompt": (c_i32, [c_vp, c_vp]),
     "nq_attend_pages_workspace_size": (c_size, [c_vp]),
@@ -127,6 +130,7 @@ _PROTOS = {
 EXPORTED = tuple(_PROTOS)
 
 _lib = None
+_front = None
 _lock = threading.Lock()
 
 
@@ -154,6 +158,23 @@ def load(path: str = LIB_PATH):
                 raise ImportError("nexusquant_b200 native library ABI mismatch")
             _lib = lib
     return _lib
+
+
+def front():
+    """The compiled front end of the serving operators (csrc/nq_front.cpp), loaded once."""
+    global _front
+    if _front is None:
+        load()
+        with _lock:
+            if _front is None:
+                if not os.path.exists(FRONT_PATH):
+                    raise ImportError(f"{FRONT_PATH} not found; build it with `make -C {os.path.join(_HERE, 'csrc')}`")
+                import torch  # noqa: F401  (its libraries first)
+                spec = importlib.util.spec_from_file_location("nq_front", FRONT_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _front = module
+    return _front
 
 
 def check(fn: str, status: int) -> None:

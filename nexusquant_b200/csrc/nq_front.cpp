@@ -1,0 +1,326 @@
+// Front end of the serving operators for PyTorch: argument checks, output and scratch allocation and
+// the call of the C entry point, in one call from Python.  A decoding step calls these for every
+// layer, and at a few tokens the host's share is what a call costs: checked and packed in Python,
+// norm_rope_qk of 4 tokens took 13.0 us a call and attend_pages of 4 sequences 10.3; here 6.4 and 5.3.
+//
+// Errors: TypeError for an unsupported dtype, ValueError for shapes that do not fit, RuntimeError for
+// tensors that are not on the GPU, NexusQuantError for a status of the C entry point.
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/extension.h>
+
+#include <cmath>
+#include <optional>
+#include <tuple>
+#include <unordered_set>
+
+#include "../../include/nexusquant_b200.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+constexpr const char* kCudaOnly = "nexusquant_b200 kernels need CUDA tensors (there is no CPU path)";
+
+int32_t i32(int64_t n) {
+  TORCH_CHECK_VALUE(n <= INT32_MAX, n, " does not fit 32 bits");
+  return (int32_t)n;
+}
+
+[[noreturn]] void fail(const char* fn, int status) {
+  pybind11::gil_scoped_acquire gil;
+  pybind11::object cls = pybind11::module_::import("nexusquant_b200._native").attr("NexusQuantError");
+  pybind11::object e = cls(fn, status);
+  PyErr_SetObject(cls.ptr(), e.ptr());
+  throw pybind11::error_already_set();
+}
+
+int dtype_code(at::ScalarType t) {
+  TORCH_CHECK_TYPE(t == at::kHalf || t == at::kBFloat16 || t == at::kFloat, "unsupported dtype ", t);
+  return t == at::kHalf ? NQ_F16 : t == at::kBFloat16 ? NQ_BF16 : NQ_F32;
+}
+
+void* stream_of(const at::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+
+// 16-byte aligned rows of contiguous elements: t itself or a contiguous copy.  Without `broadcast` a
+// stride of 0 is written out too (the copies to shared memory go by strides).
+struct Rows {
+  Tensor t;
+  void* p;
+  int64_t s0, s1;
+};
+bool rows_ok(const Tensor& t, bool broadcast) {
+  const int64_t per = 16 / t.element_size();
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.stride(2) == 1 && t.stride(0) % per == 0 &&
+         t.stride(1) % per == 0 && (broadcast || (t.stride(0) && t.stride(1)));
+}
+Rows rows16(const Tensor& t, bool broadcast) {
+  Tensor r = rows_ok(t, broadcast) ? t : t.clone(at::MemoryFormat::Contiguous);
+  return Rows{r, r.data_ptr(), r.stride(0), r.stride(1)};
+}
+
+Tensor int32(const Tensor& t, const at::Device& dev) {
+  if (t.scalar_type() == at::kInt && t.device() == dev && t.is_contiguous()) return t;
+  return t.to(dev, at::kInt).contiguous();
+}
+
+Rows output(const OptTensor& out, const Tensor& like, at::IntArrayRef shape) {
+  if (!out) {
+    Tensor t = at::empty(shape, like.options());
+    return Rows{t, t.data_ptr(), shape[1] * shape[2], shape[2]};
+  }
+  const Tensor& t = *out;
+  TORCH_CHECK_VALUE(t.sizes() == shape && t.scalar_type() == like.scalar_type() && t.device() == like.device(),
+                    "out must have the queries' shape, dtype and device");
+  bool apart = rows_ok(t, true);
+  for (int i = 0; i < 3; ++i) apart = apart && (t.stride(i) != 0 || t.size(i) <= 1);
+  TORCH_CHECK_VALUE(apart, "out needs 16-byte aligned rows of contiguous elements that do not overlap");
+  return Rows{t, t.data_ptr(), t.stride(0), t.stride(1)};
+}
+
+bool head_dim_ok(int64_t d) { return d == 64 || d == 96 || d == 128; }
+
+// q [n, hq, d], k / v [m, h, d] on one device, of one dtype, hq a multiple of h
+void check_qkv(const Tensor& q, const Tensor& k, const Tensor* v, bool f32) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && (!v || v->is_cuda()), kCudaOnly);
+  TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type() && k.device() == q.device() &&
+                        (!v || (v->scalar_type() == q.scalar_type() && v->device() == q.device())),
+                    "queries, keys and values must share dtype and device");
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && q.size(2) == k.size(2),
+                    "queries, keys and values must be [tokens, heads, head_dim] with one head_dim");
+  dtype_code(q.scalar_type());
+  TORCH_CHECK_TYPE(f32 || q.scalar_type() != at::kFloat, "unsupported dtype ", q.scalar_type());
+  TORCH_CHECK_VALUE(head_dim_ok(q.size(2)), "head_dim must be one of (64, 96, 128) (got ", q.size(2), ")");
+  TORCH_CHECK_VALUE(k.size(1) > 0 && q.size(1) > 0 && q.size(1) % k.size(1) == 0, q.size(1),
+                    " query heads are not a multiple of ", k.size(1), " KV heads");
+  TORCH_CHECK_VALUE(!v || v->sizes() == k.sizes(), "keys ", k.sizes(), " and values ", v ? v->sizes() : k.sizes(),
+                    " differ");
+}
+
+// pages [(layers,) n_pages, heads, page_size, head_dim], contiguous, keys and values alike
+void check_pages(const Tensor& k, const Tensor& v, int64_t dims) {
+  TORCH_CHECK(k.is_cuda() && v.is_cuda(), kCudaOnly);
+  TORCH_CHECK_VALUE(k.dim() == dims && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() &&
+                        k.device() == v.device(),
+                    "key and value pages must share shape, dtype and device");
+  TORCH_CHECK_VALUE(k.is_contiguous() && v.is_contiguous(), "pages must be contiguous");
+  dtype_code(k.scalar_type());
+  const int64_t page = k.size(-2);
+  TORCH_CHECK_VALUE(page == 16 || page == 32 || page == 64 || page == 128,
+                    "page size must be one of (16, 32, 64, 128) (got ", page, ")");
+  TORCH_CHECK_VALUE(head_dim_ok(k.size(-1)), "head_dim must be one of (64, 96, 128) (got ", k.size(-1), ")");
+}
+
+float logit_scale(std::optional<double> scale) {
+  if (!scale) return 0.0f;
+  TORCH_CHECK_VALUE(*scale > 0.0 && std::isfinite(*scale), "scale must be positive and finite (got ", *scale, ")");
+  return (float)*scale;
+}
+
+std::tuple<Tensor, OptTensor> norm_rope_qk(const Tensor& q, const Tensor& k, const Tensor& positions, OptTensor wq,
+                                           OptTensor wk, double eps, const OptTensor& v, const OptTensor& k_pages,
+                                           const OptTensor& v_pages, const OptTensor& slots, const Tensor& cos,
+                                           const Tensor& sin, const OptTensor& q_out, const OptTensor& k_out) {
+  const int64_t n = q.size(0), h = k.size(1), d = q.size(2);
+  const at::Device dev = q.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  nq_norm_rope_params_t p = {};
+  Rows kd{}, vr{};
+  Tensor sl;
+  if (k_pages) {  // with v_pages, v and slots: see check_norm_rope_qk
+    vr = rows16(*v, true);
+    sl = int32(*slots, dev);
+    p.v = vr.p; p.v_stride_t = vr.s0; p.v_stride_h = vr.s1;
+    p.k_pages = k_pages->data_ptr(); p.v_pages = v_pages->data_ptr();
+    p.n_pages = i32(k_pages->size(0)); p.page_size = i32(k_pages->size(2));
+    p.slots = sl.data_ptr<int32_t>();
+  } else {
+    kd = output(k_out, k, {n, h, d});
+    p.k_out = kd.p; p.ko_stride_t = kd.s0; p.ko_stride_h = kd.s1;
+  }
+  bool w32 = q.scalar_type() == at::kFloat;
+  for (const OptTensor* w : {&wq, &wk}) w32 = w32 || (*w && (*w)->scalar_type() != q.scalar_type());
+  for (OptTensor* w : {&wq, &wk}) {
+    if (!*w) continue;
+    if (w32) *w = (*w)->to(at::kFloat);
+    if (!(*w)->is_contiguous() || reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 16)
+      *w = (*w)->clone(at::MemoryFormat::Contiguous);
+  }
+  const Rows qr = rows16(q, true), kr = rows16(k, true), qo = output(q_out, q, q.sizes());
+  const Tensor pos = int32(positions, dev);
+  p.dtype = dtype_code(q.scalar_type());
+  p.tokens = i32(n); p.q_heads = i32(q.size(1)); p.heads = i32(h); p.head_dim = i32(d);
+  p.q = qr.p; p.q_stride_t = qr.s0; p.q_stride_h = qr.s1;
+  p.k = kr.p; p.k_stride_t = kr.s0; p.k_stride_h = kr.s1;
+  p.q_weight = wq ? wq->data_ptr() : nullptr;
+  p.k_weight = wk ? wk->data_ptr() : nullptr;
+  p.weight_f32 = w32; p.eps = (float)eps;
+  p.positions = pos.data_ptr<int32_t>();
+  p.rope_cos = cos.data_ptr<float>(); p.rope_sin = sin.data_ptr<float>(); p.rope_rows = i32(cos.size(0));
+  p.q_out = qo.p; p.qo_stride_t = qo.s0; p.qo_stride_h = qo.s1;
+  const nq_status_t st = nq_norm_rope_qk(&p, stream_of(dev));
+  if (st != NQ_OK) fail("nq_norm_rope_qk", st);
+  return {qo.t, k_pages ? OptTensor() : OptTensor(kd.t)};
+}
+
+// the checks of norm_rope_qk, before the rotation table is looked up
+void check_norm_rope_qk(const Tensor& q, const Tensor& k, const Tensor& positions, const OptTensor& wq,
+                        const OptTensor& wk, const OptTensor& v, const OptTensor& k_pages, const OptTensor& v_pages,
+                        const OptTensor& slots) {
+  check_qkv(q, k, v ? &*v : nullptr, true);
+  const int64_t n = q.size(0);
+  TORCH_CHECK_VALUE(k.size(0) == n && positions.numel() == n, k.size(0), " keys and ", positions.numel(),
+                    " positions for ", n, " queries");
+  if (k_pages || v_pages) {
+    TORCH_CHECK_VALUE(k_pages && v_pages && v && slots, "storing into pages needs k_pages, v_pages, v and slots");
+    check_pages(*k_pages, *v_pages, 4);
+    TORCH_CHECK_VALUE(k_pages->scalar_type() == q.scalar_type() && k_pages->device() == q.device() &&
+                          k_pages->size(1) == k.size(1) && k_pages->size(3) == q.size(2),
+                      "pages must have the keys' dtype, device, heads and head_dim");
+    TORCH_CHECK_VALUE(slots->numel() == n, slots->numel(), " slots for ", n, " tokens");
+  } else {
+    TORCH_CHECK_VALUE(!slots, "slots need pages");
+  }
+  for (const OptTensor* w : {&wq, &wk})
+    TORCH_CHECK_VALUE(!*w || ((*w)->numel() == q.size(2) && (*w)->device() == q.device()),
+                      "norm weights must be [head_dim] on the queries' device");
+}
+
+std::tuple<Tensor, OptTensor> attend_prompt(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& seq_starts,
+                                            const OptTensor& k_starts, std::optional<double> scale,
+                                            const OptTensor& out, bool return_lse) {
+  check_qkv(q, k, &v, false);
+  const at::Device dev = q.device();
+  const int64_t n = q.size(0), m = k.size(0), hq = q.size(1);
+  TORCH_CHECK_VALUE(seq_starts.dim() == 1 && seq_starts.numel() >= 1, "seq_starts must be [n_seqs + 1]");
+  TORCH_CHECK_VALUE(k_starts || m == n, m, " keys for ", n, " queries: give k_starts");
+  TORCH_CHECK_VALUE(!k_starts || k_starts->sizes() == seq_starts.sizes(),
+                    "k_starts and seq_starts must have the same shape");
+  const c10::cuda::CUDAGuard guard(dev);
+  nq_attend_prompt_params_t p = {};
+  p.scale = logit_scale(scale);
+  const Tensor st = int32(seq_starts, dev), kst = k_starts ? int32(*k_starts, dev) : st;
+  const Rows qr = rows16(q, false), kr = rows16(k, false), vr = rows16(v, false), o = output(out, q, q.sizes());
+  OptTensor lse;
+  if (return_lse) lse = at::empty({n, hq}, q.options().dtype(at::kFloat));
+  p.dtype = dtype_code(q.scalar_type());
+  p.n_seqs = i32(st.numel() - 1); p.q_tokens = i32(n); p.k_tokens = i32(m);
+  p.q_heads = i32(hq); p.heads = i32(k.size(1)); p.head_dim = i32(q.size(2));
+  p.q = qr.p; p.q_stride_t = qr.s0; p.q_stride_h = qr.s1;
+  p.k = kr.p; p.k_stride_t = kr.s0; p.k_stride_h = kr.s1;
+  p.v = vr.p; p.v_stride_t = vr.s0; p.v_stride_h = vr.s1;
+  p.seq_starts = st.data_ptr<int32_t>(); p.k_starts = kst.data_ptr<int32_t>();
+  p.out = o.p; p.o_stride_t = o.s0; p.o_stride_h = o.s1;
+  p.lse = lse ? lse->data_ptr<float>() : nullptr;
+  const nq_status_t rc = nq_attend_prompt(&p, stream_of(dev));
+  if (rc != NQ_OK) fail("nq_attend_prompt", rc);
+  return {o.t, lse};
+}
+
+Tensor attend_pages(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables,
+                    const Tensor& lens, const OptTensor& prefix_table, int64_t prefix_len,
+                    std::optional<int64_t> max_len, std::optional<double> scale, const OptTensor& out) {
+  TORCH_CHECK_VALUE(q.dim() == 3, "queries must be [batch, heads, head_dim]");
+  check_pages(k_pages, v_pages, 4);
+  TORCH_CHECK(q.is_cuda(), kCudaOnly);
+  TORCH_CHECK_TYPE(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "unsupported dtype ",
+                   q.scalar_type());
+  const at::Device dev = q.device();
+  const int64_t b = q.size(0), hq = q.size(1), d = q.size(2), h = k_pages.size(1), page = k_pages.size(2);
+  TORCH_CHECK_VALUE(q.scalar_type() == k_pages.scalar_type() && dev == k_pages.device() && d == k_pages.size(3),
+                    "queries and pages must share dtype, device and head_dim");
+  TORCH_CHECK_VALUE(h > 0 && hq > 0 && hq % h == 0, hq, " query heads are not a multiple of ", h, " KV heads");
+  TORCH_CHECK_VALUE(tables.dim() == 2 && tables.size(0) == b && lens.numel() == b, "tables must be [", b,
+                    ", width] and lens [", b, "]");
+  const int64_t holds = tables.size(1) * page, most = max_len ? *max_len : holds;
+  TORCH_CHECK_VALUE(0 <= most && most <= holds, "max_len ", most, " outside the tables' ", holds, " tokens");
+  TORCH_CHECK_VALUE(prefix_len == 0 || (prefix_len > 0 && prefix_table && prefix_table->numel() * page >= prefix_len),
+                    "prefix_table does not hold ", prefix_len, " tokens");
+  const c10::cuda::CUDAGuard guard(dev);
+  nq_attend_pages_params_t p = {};
+  p.scale = logit_scale(scale);
+  const Tensor tb = int32(tables, dev), ln = int32(lens, dev);
+  Tensor pre;
+  if (prefix_len) pre = int32(*prefix_table, dev);
+  const Rows qr = rows16(q, false), o = output(out, q, q.sizes());
+  p.dtype = dtype_code(q.scalar_type());
+  p.batch = i32(b); p.q_heads = i32(hq); p.heads = i32(h); p.head_dim = i32(d);
+  p.n_pages = i32(k_pages.size(0)); p.page_size = i32(page);
+  p.q = qr.p; p.q_stride_b = qr.s0; p.q_stride_h = qr.s1;
+  p.k_pages = k_pages.data_ptr(); p.v_pages = v_pages.data_ptr();
+  p.tables = tb.data_ptr<int32_t>(); p.table_width = i32(tb.size(1));
+  p.lens = ln.data_ptr<int32_t>(); p.max_len = i32(most);
+  p.prefix_table = prefix_len ? pre.data_ptr<int32_t>() : nullptr; p.prefix_len = i32(prefix_len);
+  p.out = o.p; p.o_stride_b = o.s0; p.o_stride_h = o.s1;
+  // scratch from torch's allocator each call: it belongs to the current stream, captured or not
+  const size_t bytes = nq_attend_pages_workspace_size(&p);
+  Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  const nq_status_t rc = nq_attend_pages(&p, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(dev));
+  if (rc != NQ_OK) fail("nq_attend_pages", rc);
+  return o.t;
+}
+
+nq_pool_t pool_of(const Tensor& k, const Tensor& v) {
+  check_pages(k, v, k.dim() == 4 ? 4 : 5);
+  return nq_pool_t{k.data_ptr(), v.data_ptr(), k.dim() == 4 ? 1 : i32(k.size(0)), i32(k.size(-4)),
+                   i32(k.size(-3)), i32(k.size(-2)), i32(k.size(-1) * k.element_size())};
+}
+
+void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& src, const Tensor& dst) {
+  const nq_pool_t pool = pool_of(k_pages, v_pages);
+  TORCH_CHECK_VALUE(src.dim() == 1 && src.sizes() == dst.sizes(), "src and dst must be [n]");
+  if (src.is_cpu() && dst.is_cpu()) {  // pairs on the device are taken as they are
+    const Tensor s = src.to(at::kLong).contiguous(), t = dst.to(at::kLong).contiguous();
+    const std::unordered_set<int64_t> from(s.data_ptr<int64_t>(), s.data_ptr<int64_t>() + s.numel());
+    const std::unordered_set<int64_t> to(t.data_ptr<int64_t>(), t.data_ptr<int64_t>() + t.numel());
+    bool twice = (int64_t)to.size() < t.numel();
+    for (const int64_t p : to) twice = twice || from.count(p);
+    TORCH_CHECK_VALUE(!twice, "a destination page is also a source or is written twice");
+    for (const auto* set : {&from, &to})
+      for (const int64_t p : *set)
+        TORCH_CHECK_VALUE(0 <= p && p < pool.n_pages, "page numbers outside the pool of ", pool.n_pages);
+  }
+  const at::Device dev = k_pages.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor s = int32(src, dev), t = int32(dst, dev);
+  const nq_status_t rc = nq_copy_pages(&pool, s.data_ptr<int32_t>(), t.data_ptr<int32_t>(), i32(s.numel()),
+                                       stream_of(dev));
+  if (rc != NQ_OK) fail("nq_copy_pages", rc);
+}
+
+void compact_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& tables, const Tensor& kept_idx,
+                   const OptTensor& kept_count, const Tensor& dst_tables, std::optional<int64_t> max_kept) {
+  const nq_pool_t pool = pool_of(k_pages, v_pages);
+  TORCH_CHECK_VALUE(tables.dim() == 2 && dst_tables.dim() == 2 && kept_idx.dim() == 2,
+                    "tables, dst_tables and kept_idx must be [batch, ...]");
+  const int64_t b = tables.size(0);
+  TORCH_CHECK_VALUE(dst_tables.size(0) == b && kept_idx.size(0) == b && (!kept_count || kept_count->numel() == b),
+                    "dst_tables, kept_idx and kept_count must have ", b, " rows");
+  const int64_t holds = std::min<int64_t>(kept_idx.size(1), dst_tables.size(1) * pool.page_size);
+  const int64_t most = max_kept ? *max_kept : holds;
+  TORCH_CHECK_VALUE(0 <= most && most <= holds, "max_kept ", most, " above the ", holds,
+                    " that kept_idx and dst_tables hold");
+  const at::Device dev = k_pages.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  const Tensor t = int32(tables, dev), i = int32(kept_idx, dev), to = int32(dst_tables, dev);
+  Tensor n;
+  if (kept_count) n = int32(*kept_count, dev);
+  const nq_status_t rc = nq_compact_pages(&pool, i32(b), t.data_ptr<int32_t>(), i32(t.size(1)), i.data_ptr<int32_t>(),
+                                          i.size(1), kept_count ? n.data_ptr<int32_t>() : nullptr, i32(most),
+                                          to.data_ptr<int32_t>(), i32(to.size(1)), stream_of(dev));
+  if (rc != NQ_OK) fail("nq_compact_pages", rc);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(nq_front, m) {
+  // without the GIL: a launch waits while the GPU's queue is full
+  m.def("check_norm_rope_qk", torch::wrap_pybind_function_no_gil(check_norm_rope_qk));
+  m.def("norm_rope_qk", torch::wrap_pybind_function_no_gil(norm_rope_qk));
+  m.def("attend_prompt", torch::wrap_pybind_function_no_gil(attend_prompt));
+  m.def("attend_pages", torch::wrap_pybind_function_no_gil(attend_pages));
+  m.def("copy_pages", torch::wrap_pybind_function_no_gil(copy_pages));
+  m.def("compact_pages", torch::wrap_pybind_function_no_gil(compact_pages));
+}

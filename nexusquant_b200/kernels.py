@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-import struct
 from dataclasses import dataclass
 from typing import List, Optional, Sequence, Union
 
@@ -656,112 +655,9 @@ def attend_compressed(q: torch.Tensor, codes: LayerCodes, positions: torch.Tenso
 # Serving operators around the cache: tensors are [tokens, heads, head_dim]
 #
 # A decoding step calls these for every layer, and at a few tokens the host's share is what a call
-# costs: parameters are packed with struct (the C structs of include/nexusquant_b200.h, native
-# alignment), and attributes of a tensor are read once.
+# costs: their checks, outputs and launches are one compiled call (csrc/nq_front.cpp).
 # ---------------------------------------------------------------------------
 PAGE_SIZES = (16, 32, 64, 128)
-_HEAD_DIMS = (64, 96, 128)
-_ATTEND_DTYPES = (torch.float16, torch.bfloat16)
-_NORM_ROPE = struct.Struct("@5i3P6q2Pif3Pi2P4q2P2iP").pack
-_ATTEND_PROMPT = struct.Struct("@7i3P6q2PfP2qP").pack
-_ATTEND_PAGES = struct.Struct("@7iP2q3PiPiPifP2q").pack
-_POOL = struct.Struct("@2P5i").pack
-_CUDA_ONLY = "nexusquant_b200 kernels need CUDA tensors (there is no CPU path)"
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-
-
-def _rows16(t: torch.Tensor, broadcast: bool = True):
-    """(t, address, strides of the two outer dimensions) with 16-byte aligned rows of contiguous
-    elements; t is a contiguous copy where its rows are not, or, unless broadcast is allowed, where a
-    stride is 0."""
-    ptr, (s0, s1, s2) = t.data_ptr(), t.stride()
-    per = 3 if t.dtype is torch.float32 else 7
-    if ptr & 15 or s2 != 1 or s0 & per or s1 & per or not (broadcast or (s0 and s1)):
-        t = t.clone(memory_format=torch.contiguous_format)
-        ptr, (s0, s1, _) = t.data_ptr(), t.stride()
-    return t, ptr, s0, s1
-
-
-def _int32(t: torch.Tensor, index: int) -> torch.Tensor:
-    if t.dtype is torch.int32 and t.get_device() == index and t.is_contiguous():
-        return t
-    return t.to(device=torch.device("cuda", index), dtype=torch.int32).contiguous()
-
-
-def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: Optional[torch.Tensor], dtypes):
-    """q [n, hq, d], k / v [m, h, d] on one device, of one dtype, hq a multiple of h, d 64, 96 or 128.
-    Returns the shapes of q and k."""
-    index, dt = q.get_device(), q.dtype
-    if index < 0 or k.get_device() < 0 or (v is not None and v.get_device() < 0):
-        raise RuntimeError(_CUDA_ONLY)
-    if k.dtype != dt or k.get_device() != index or (v is not None and (v.dtype != dt or v.get_device() != index)):
-        raise ValueError("queries, keys and values must share dtype and device")
-    qs, ks = q.shape, k.shape
-    if len(qs) != 3 or len(ks) != 3 or qs[2] != ks[2]:
-        raise ValueError("queries, keys and values must be [tokens, heads, head_dim] with one head_dim")
-    if dt not in dtypes:
-        raise TypeError(f"unsupported dtype {dt}")
-    if qs[2] not in _HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {_HEAD_DIMS} (got {qs[2]})")
-    if ks[1] == 0 or qs[1] == 0 or qs[1] % ks[1]:
-        raise ValueError(f"{qs[1]} query heads are not a multiple of {ks[1]} KV heads")
-    if v is not None and v.shape != ks:
-        raise ValueError(f"keys {tuple(ks)} and values {tuple(v.shape)} differ")
-    return qs, ks
-
-
-def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dims: int):
-    """Pages [(layers,) n_pages, heads, page_size, head_dim], contiguous, keys and values alike.
-    Returns their shape."""
-    index, shape = k_pages.get_device(), k_pages.shape
-    if index < 0 or v_pages.get_device() < 0:
-        raise RuntimeError(_CUDA_ONLY)
-    if len(shape) != dims or shape != v_pages.shape or k_pages.dtype != v_pages.dtype or index != v_pages.get_device():
-        raise ValueError("key and value pages must share shape, dtype and device")
-    if not k_pages.is_contiguous() or not v_pages.is_contiguous():
-        raise ValueError("pages must be contiguous")
-    if k_pages.dtype not in _DTYPES:
-        raise TypeError(f"unsupported dtype {k_pages.dtype}")
-    if shape[-2] not in PAGE_SIZES:
-        raise ValueError(f"page size must be one of {PAGE_SIZES} (got {shape[-2]})")
-    if shape[-1] not in _HEAD_DIMS:
-        raise ValueError(f"head_dim must be one of {_HEAD_DIMS} (got {shape[-1]})")
-    return shape
-
-
-def _out(out: Optional[torch.Tensor], like: torch.Tensor, shape):
-    """(out, address, outer strides): a new tensor of the given shape, or the caller's, checked."""
-    if out is None:
-        out = like.new_empty(shape)
-        return out, out.data_ptr(), shape[1] * shape[2], shape[2]
-    if out.shape != shape or out.dtype != like.dtype or out.get_device() != like.get_device():
-        raise ValueError("out must have the queries' shape, dtype and device")
-    same, ptr, s0, s1 = _rows16(out)
-    if same is not out or any(st == 0 and n > 1 for st, n in zip(out.stride(), shape)):
-        raise ValueError("out needs 16-byte aligned rows of contiguous elements that do not overlap")
-    return out, ptr, s0, s1
-
-
-def _logit_scale(scale: Optional[float]) -> float:
-    """0 for the default 1 / sqrt(head_dim), else a positive number."""
-    if scale is None:
-        return 0.0
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite (got {scale})")
-    return float(scale)
-
-
-def _launch(index: int, fn: str, *args) -> None:
-    """Call an entry point on device ``index``'s current stream, with that device current."""
-    entry = getattr(N.load(), fn)
-    if _raw_device() == index:
-        status = entry(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            status = entry(*args, _raw_stream(index))
-    if status:
-        N.check(fn, status)
 
 
 def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *,
@@ -782,58 +678,13 @@ def norm_rope_qk(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, *,
     rope_rows : RoPE table rows to use when every position is known to be below it; None reads
                 positions.max() (a host synchronisation) to size the table.
     Returns (q_out, k_out); k_out is None with pages.  Computed in fp32, rounded once."""
-    (n, hq, d), (nk, h, _) = _check_qkv(q, k, v, _DTYPES)
-    index, dt = q.get_device(), q.dtype
-    if nk != n or positions.numel() != n:
-        raise ValueError(f"{nk} keys and {positions.numel()} positions for {n} queries")
-    ko = kos0 = kos1 = vp = vs0 = vs1 = kp = vpp = n_pages = page = slot_p = 0
-    if k_pages is not None or v_pages is not None:
-        if k_pages is None or v_pages is None or v is None or slots is None:
-            raise ValueError("storing into pages needs k_pages, v_pages, v and slots")
-        n_pages, hp, page, dp = _check_pages(k_pages, v_pages, 4)
-        if k_pages.dtype != dt or k_pages.get_device() != index or hp != h or dp != d:
-            raise ValueError("pages must have the keys' dtype, device, heads and head_dim")
-        if slots.numel() != n:
-            raise ValueError(f"{slots.numel()} slots for {n} tokens")
-        slots = _int32(slots, index)
-        v, vp, vs0, vs1 = _rows16(v)
-        k_out, kp, vpp, slot_p = None, k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr()
-    elif slots is not None:
-        raise ValueError("slots need pages")
-    else:
-        k_out, ko, kos0, kos1 = _out(k_out, k, (n, h, d))
-    w32 = False
-    for w in (q_weight, k_weight):
-        if w is not None:
-            if w.numel() != d or w.get_device() != index:
-                raise ValueError("norm weights must be [head_dim] on the queries' device")
-            w32 = w32 or w.dtype != dt
-    if w32:
-        q_weight, k_weight = (None if w is None else w.float() for w in (q_weight, k_weight))
-    wq = wk = 0
-    if q_weight is not None:
-        q_weight = _weight16(q_weight)
-        wq = q_weight.data_ptr()
-    if k_weight is not None:
-        k_weight = _weight16(k_weight)
-        wk = k_weight.data_ptr()
-    q, qp, qs0, qs1 = _rows16(q)
-    k, kptr, ks0, ks1 = _rows16(k)
-    positions = _int32(positions, index)
+    front = N.front()
+    front.check_norm_rope_qk(q, k, positions, q_weight, k_weight, v, k_pages, v_pages, slots)
     if rope_rows is None:
-        rope_rows = int(positions.max().item()) + 1 if n else 1
-    cos, sin = TABLES.get(q.device, d, rope_base, int(rope_rows), rope_scaling)
-    q_out, qo, qos0, qos1 = _out(q_out, q, (n, hq, d))
-    _launch(index, "nq_norm_rope_qk", _NORM_ROPE(
-        _DTYPES[dt], n, hq, h, d, qp, kptr, vp, qs0, qs1, ks0, ks1, vs0, vs1, wq, wk,
-        int(w32 or dt == torch.float32), eps, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-        qo, ko, qos0, qos1, kos0, kos1, kp, vpp, n_pages, page, slot_p))
-    return q_out, k_out
-
-
-def _weight16(w: torch.Tensor) -> torch.Tensor:
-    """A norm weight of contiguous elements at a 16-byte boundary."""
-    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+        rope_rows = int(positions.max().item()) + 1 if positions.numel() else 1
+    cos, sin = TABLES.get(q.device, q.shape[2], rope_base, int(rope_rows), rope_scaling)
+    return front.norm_rope_qk(q, k, positions, q_weight, k_weight, eps, v, k_pages, v_pages, slots, cos, sin, q_out,
+                              k_out)
 
 
 def attend_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts: torch.Tensor, *,
@@ -849,29 +700,7 @@ def attend_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_starts:
     Returns [n, hq, d] (and, with return_lse, the fp32 log of the softmax sums [n, hq]).  A query that
     sees no key gets zeros and -inf; keys that a query does not see never reach its row; rows of no
     sequence are not written."""
-    (n, hq, d), (m, h, _) = _check_qkv(q, k, v, _ATTEND_DTYPES)
-    index, dt = q.get_device(), q.dtype
-    if seq_starts.dim() != 1 or seq_starts.numel() < 1:
-        raise ValueError("seq_starts must be [n_seqs + 1]")
-    seq_starts = _int32(seq_starts, index)
-    if k_starts is None:
-        if m != n:
-            raise ValueError(f"{m} keys for {n} queries: give k_starts")
-        k_starts = seq_starts
-    else:
-        if k_starts.shape != seq_starts.shape:
-            raise ValueError("k_starts and seq_starts must have the same shape")
-        k_starts = _int32(k_starts, index)
-    # the copies to shared memory go by strides: tensors broadcast over heads or tokens are written out
-    q, qp, qs0, qs1 = _rows16(q, False)
-    k, kp, ks0, ks1 = _rows16(k, False)
-    v, vp, vs0, vs1 = _rows16(v, False)
-    out, op, os0, os1 = _out(out, q, (n, hq, d))
-    lse = q.new_empty((n, hq), dtype=torch.float32) if return_lse else None
-    _launch(index, "nq_attend_prompt", _ATTEND_PROMPT(
-        _DTYPES[dt], seq_starts.numel() - 1, n, m, hq, h, d, qp, kp, vp, qs0, qs1, ks0, ks1, vs0, vs1,
-        seq_starts.data_ptr(), k_starts.data_ptr(), _logit_scale(scale), op, os0, os1,
-        0 if lse is None else lse.data_ptr()))
+    out, lse = N.front().attend_prompt(q, k, v, seq_starts, k_starts, scale, out, return_lse)
     return (out, lse) if return_lse else out
 
 
@@ -888,51 +717,7 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
                    read once for the whole batch.
     max_len      : bound on lens (a host number); None: width * page_size.
     Returns [b, hq, d]; a sequence without any token gets zeros."""
-    if q.dim() != 3:
-        raise ValueError("queries must be [batch, heads, head_dim]")
-    n_pages, h, page, dp = _check_pages(k_pages, v_pages, 4)
-    b, hq, d = q.shape
-    index, dt = q.get_device(), q.dtype
-    if index < 0:
-        raise RuntimeError(_CUDA_ONLY)
-    if dt not in _ATTEND_DTYPES:
-        raise TypeError(f"unsupported dtype {dt}")
-    if dt != k_pages.dtype or index != k_pages.get_device() or d != dp:
-        raise ValueError("queries and pages must share dtype, device and head_dim")
-    if h == 0 or hq == 0 or hq % h:
-        raise ValueError(f"{hq} query heads are not a multiple of {h} KV heads")
-    if tables.dim() != 2 or tables.shape[0] != b or lens.numel() != b:
-        raise ValueError(f"tables must be [{b}, width] and lens [{b}]")
-    width = tables.shape[1]
-    if max_len is None:
-        max_len = width * page
-    if not 0 <= max_len <= width * page:
-        raise ValueError(f"max_len {max_len} outside the tables' {width * page} tokens")
-    pre = 0
-    if prefix_len:
-        if prefix_len < 0 or prefix_table is None or prefix_table.numel() * page < prefix_len:
-            raise ValueError(f"prefix_table does not hold {prefix_len} tokens")
-        prefix_table = _int32(prefix_table, index)
-        pre = prefix_table.data_ptr()
-    tables, lens = _int32(tables, index), _int32(lens, index)
-    q, qp, qs0, qs1 = _rows16(q, False)
-    out, op, os0, os1 = _out(out, q, (b, hq, d))
-    p = _ATTEND_PAGES(_DTYPES[dt], b, hq, h, d, n_pages, page, qp, qs0, qs1, k_pages.data_ptr(), v_pages.data_ptr(),
-                      tables.data_ptr(), width, lens.data_ptr(), max_len, pre, prefix_len, _logit_scale(scale), op, os0,
-                      os1)
-    nbytes = N.load().nq_attend_pages_workspace_size(p)
-    # scratch from torch's allocator each call: it belongs to the current stream, captured or not
-    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-    _launch(index, "nq_attend_pages", p, 0 if ws is None else ws.data_ptr(), nbytes)
-    return out
-
-
-def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor):
-    """(packed nq_pool_t, pages, page size) of [layers, ...] pages or of one layer's."""
-    shape = _check_pages(k_pages, v_pages, 4 if k_pages.dim() == 4 else 5)
-    layers, (n_pages, h, page, d) = (1 if len(shape) == 4 else shape[0]), shape[-4:]
-    return (_POOL(k_pages.data_ptr(), v_pages.data_ptr(), layers, n_pages, h, page, d * k_pages.element_size()),
-            n_pages, page)
+    return N.front().attend_pages(q, k_pages, v_pages, tables, lens, prefix_table, prefix_len, max_len, scale, out)
 
 
 def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -941,18 +726,7 @@ def copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: torch.Tensor, 
     k_pages, v_pages : [layers, n_pages, h, page_size, d] (or one layer's 4-D pages).
     src, dst         : int32 [n].  No page of dst may be in src or twice in dst: pairs given on
                        the CPU are checked, those on the device are taken as they are."""
-    pool, n_pages, _ = _pool(k_pages, v_pages)
-    if src.shape != dst.shape or src.dim() != 1:
-        raise ValueError("src and dst must be [n]")
-    if not src.is_cuda and not dst.is_cuda:
-        s, t = src.tolist(), dst.tolist()
-        if len(set(t)) < len(t) or set(s) & set(t):
-            raise ValueError("a destination page is also a source or is written twice")
-        if s and not (0 <= min(s + t) and max(s + t) < n_pages):
-            raise ValueError(f"page numbers outside the pool of {n_pages}")
-    index = k_pages.get_device()
-    src, dst = _int32(src, index), _int32(dst, index)
-    _launch(index, "nq_copy_pages", pool, src.data_ptr(), dst.data_ptr(), src.numel())
+    N.front().copy_pages(k_pages, v_pages, src, dst)
 
 
 def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor, kept_idx: torch.Tensor,
@@ -966,20 +740,4 @@ def compact_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Te
     kept_idx, kept_count : as select_keep returns them (int32 [b, T] ascending, [b]); None: max_kept each.
     max_kept             : bound on kept_count (a host number); None: what kept_idx and the fresh pages
                            can hold."""
-    pool, _, page = _pool(k_pages, v_pages)
-    if tables.dim() != 2 or dst_tables.dim() != 2 or kept_idx.dim() != 2:
-        raise ValueError("tables, dst_tables and kept_idx must be [batch, ...]")
-    b = tables.shape[0]
-    if dst_tables.shape[0] != b or kept_idx.shape[0] != b or (kept_count is not None and kept_count.numel() != b):
-        raise ValueError(f"dst_tables, kept_idx and kept_count must have {b} rows")
-    holds = min(kept_idx.shape[1], dst_tables.shape[1] * page)
-    if max_kept is None:
-        max_kept = holds
-    if not 0 <= max_kept <= holds:
-        raise ValueError(f"max_kept {max_kept} above the {holds} that kept_idx and dst_tables hold")
-    index = k_pages.get_device()
-    tables, dst_tables, kept_idx = _int32(tables, index), _int32(dst_tables, index), _int32(kept_idx, index)
-    kept_count = None if kept_count is None else _int32(kept_count, index)
-    _launch(index, "nq_compact_pages", pool, b, tables.data_ptr(), tables.shape[1], kept_idx.data_ptr(),
-            kept_idx.shape[1], 0 if kept_count is None else kept_count.data_ptr(),
-            int(max_kept), dst_tables.data_ptr(), dst_tables.shape[1])
+    N.front().compact_pages(k_pages, v_pages, tables, kept_idx, kept_count, dst_tables, max_kept)

@@ -12,6 +12,7 @@ Tolerances.  u is the unit roundoff of the tensors' type (2^-11 fp16, 2^-8 bf16,
     (sum_i |q_i k_i| scale <= 32 in fp32 with 128 terms: at most 128 * 2^-24 * 32 = 2^-12 in the
     worst case, and far from all roundings have one sign)."""
 import math
+import struct
 
 import pytest
 import torch
@@ -685,6 +686,11 @@ PROMPT_FIELDS = """dtype n_seqs q_tokens k_tokens q_heads heads head_dim q k v q
     v_stride_t v_stride_h seq_starts k_starts scale out o_stride_t o_stride_h lse""".split()
 PAGES_FIELDS = """dtype batch q_heads heads head_dim n_pages page_size q q_stride_b q_stride_h k_pages v_pages tables
     table_width lens max_len prefix_table prefix_len scale out o_stride_b o_stride_h""".split()
+# and their native layout
+NORM_ROPE_PACK = struct.Struct("@5i3P6q2Pif3Pi2P4q2P2iP").pack
+ATTEND_PROMPT_PACK = struct.Struct("@7i3P6q2PfP2qP").pack
+ATTEND_PAGES_PACK = struct.Struct("@7iP2q3PiPiPifP2q").pack
+POOL_PACK = struct.Struct("@2P5i").pack
 
 
 def test_entry_points_refuse_without_a_gpu():
@@ -698,7 +704,7 @@ def test_entry_points_refuse_without_a_gpu():
             return call(pack(*[{**base, **kw}.get(f, 0) for f in fields]))
         return run
 
-    rope = maker(ROPE_FIELDS, K._NORM_ROPE, lambda p: lib.nq_norm_rope_qk(p, None), dtype=0, tokens=2, q_heads=4, heads=2,
+    rope = maker(ROPE_FIELDS, NORM_ROPE_PACK, lambda p: lib.nq_norm_rope_qk(p, None), dtype=0, tokens=2, q_heads=4, heads=2,
                  head_dim=128, q=one, k=one, q_out=one, k_out=one, positions=one, rope_cos=one, rope_sin=one, rope_rows=8)
     assert lib.nq_norm_rope_qk(None, None) == -1
     assert rope(tokens=0) == 0 and rope(tokens=-1) == -1 and rope(head_dim=80) == -2 and rope(dtype=3) == -1
@@ -706,14 +712,14 @@ def test_entry_points_refuse_without_a_gpu():
     assert rope(k_pages=one) == -1 and rope(k_pages=one, v_pages=one, page_size=48) == -2
     assert rope(k_pages=one, v_pages=one, page_size=16) == -1  # no v, no slots
 
-    prompt = maker(PROMPT_FIELDS, K._ATTEND_PROMPT, lambda p: lib.nq_attend_prompt(p, None), dtype=0, n_seqs=1, q_tokens=2,
+    prompt = maker(PROMPT_FIELDS, ATTEND_PROMPT_PACK, lambda p: lib.nq_attend_prompt(p, None), dtype=0, n_seqs=1, q_tokens=2,
                    k_tokens=2, q_heads=4, heads=2, head_dim=128, q=one, k=one, v=one, seq_starts=one, k_starts=one, out=one)
     assert lib.nq_attend_prompt(None, None) == -1
     assert prompt(q_tokens=0) == 0 and prompt(n_seqs=0) == 0 and prompt(dtype=2) == -2 and prompt(head_dim=32) == -2
     assert prompt(q_heads=3) == -2 and prompt(out=0) == -1 and prompt(seq_starts=0) == -1 and prompt(scale=-0.5) == -1
     assert prompt(v=one + 2) == -6 and prompt(k_stride_h=12) == -6
 
-    pages = maker(PAGES_FIELDS, K._ATTEND_PAGES, lambda p: lib.nq_attend_pages(p, None, 0, None), dtype=0, batch=1,
+    pages = maker(PAGES_FIELDS, ATTEND_PAGES_PACK, lambda p: lib.nq_attend_pages(p, None, 0, None), dtype=0, batch=1,
                   q_heads=4, heads=2, head_dim=128, n_pages=4, page_size=16, q=one, k_pages=one, v_pages=one, tables=one,
                   table_width=2, lens=one, max_len=32, out=one)
     assert lib.nq_attend_pages(None, None, 0, None) == -1 and lib.nq_attend_pages_workspace_size(None) == 0
@@ -722,7 +728,7 @@ def test_entry_points_refuse_without_a_gpu():
     assert pages(max_len=32, batch=4096, scale=math.inf) == -1
 
     def pool(page=16, row=256):
-        return K._POOL(one, one, 2, 4, 2, page, row)
+        return POOL_PACK(one, one, 2, 4, 2, page, row)
 
     assert lib.nq_copy_pages(None, one, one, 1, None) == -1 and lib.nq_copy_pages(pool(), one, one, 0, None) == 0
     assert lib.nq_copy_pages(pool(), None, one, 1, None) == -1
