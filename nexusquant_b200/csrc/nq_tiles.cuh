@@ -207,7 +207,7 @@ struct Half16<__nv_bfloat16> {
 
 // TMEM columns.  At D = 64 the weights P have columns of their own (kAhead): S is free as soon as the
 // softmax warps have read it, and the next S is computed while they work on this one (16384 tokens of
-// 32 / 8 heads 1311 -> 1235 us).  At D = 96 and 128 there is no room for that.
+// 32 / 8 heads 1311 -> 1240 us, with kPoly = 2 before and after).  At D = 96 and 128 there is no room for that.
 template <int D>
 struct TileTmem {
   static constexpr bool kAhead = D <= 64;
@@ -289,15 +289,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   constexpr bool AHEAD = Tm::kAhead;
   constexpr int NST = Lo::kStages;
   // Of 8 exponentials, how many the multiply-add pipe computes.  A tile at d = 64 has half the products
-  // per exponential: there 2 of 8 take 16384 tokens of 32 heads from 1428 to 1346 us
-  // (4 of 8: 1380).  At d = 96 and 128 they only cost power: 457 -> 461 us, 1669 -> 1683 us.
-  constexpr int kPoly = D == 64 ? 2 : 0;
+  // per exponential: there 1 of 8 takes 16384 tokens of 32 heads from 1263 to 1200 us
+  // (2 of 8: 1240, 3: 1268).  At d = 96 and 128 they only cost power (2 of 8: 457 -> 461 us, 1669 -> 1683 us).
+  constexpr int kPoly = D == 64 ? 1 : 0;
   extern __shared__ __align__(1024) uint8_t sm[];  // the 128-byte swizzle counts from multiples of 1024
   uint8_t* ring = sm + Lo::kQ;
   float2* ml_s = reinterpret_cast<float2*>(ring + NST * Lo::kItem);
   __shared__ alignas(16) uint4 clc_s;
-  __shared__ uint64_t full[NST], empty[NST], qfull, qfree, sfull[2], sread[2], pready[2], pvdone[2], odone[2], vraw[8], scrubbed[8], drain,
-      jfull[2], jfree[2], clc, xfull, xfree;
+  __shared__ uint64_t full[NST], empty[NST], qfull, qfree, sfull[2], sread[2], pready[2], pvdone[2], odone[2], vraw[8],
+      scrubbed[8], drain, jfull[2], jfree[2], clc, xfull, xfree;
   __shared__ uint32_t tmem_base, bad_keys[2][8];
   __shared__ int err;
   __shared__ TileJob job_s[2];
