@@ -288,10 +288,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   using Tm = TileTmem<D>;
   constexpr bool AHEAD = Tm::kAhead;
   constexpr int NST = Lo::kStages;
-  // Of 8 exponentials, how many the multiply-add pipe computes.  A tile at d = 64 has half the products
-  // per exponential: there 1 of 8 takes 16384 tokens of 32 heads from 1263 to 1200 us
-  // (2 of 8: 1240, 3: 1268).  At d = 96 and 128 they only cost power (2 of 8: 457 -> 461 us, 1669 -> 1683 us).
-  constexpr int kPoly = D == 64 ? 1 : 0;
+  // Of 8 exponentials, how many the multiply-add pipe computes, with none -> 1 (32 / 8 heads): d = 64, 16384
+  // tokens 1263 -> 1205 us; d = 96, 8192 tokens 385 -> 378; d = 128, 4096 tokens 116.5 -> 115.4, 16384 tokens
+  // 1811 -> 1791, within the spread of a power-capped run.  More cost power and issue slots: 2 of 8 take 1240 us
+  // at d = 64, 3 take 1268.
+  constexpr int kPoly = 1;
   extern __shared__ __align__(1024) uint8_t sm[];  // the 128-byte swizzle counts from multiples of 1024
   uint8_t* ring = sm + Lo::kQ;
   float2* ml_s = reinterpret_cast<float2*>(ring + NST * Lo::kItem);
